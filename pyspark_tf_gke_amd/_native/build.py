@@ -64,8 +64,10 @@ def build_hip(force: bool = False, jobs: int = 8, verbose: bool = True, checked:
     out_lib = HIP_LIB_CHECKED if checked else (HERE / f"libptg_hip_{variant}.so" if variant else HIP_LIB)
     bdir.mkdir(parents=True, exist_ok=True)
     hipcc = _hipcc()
+    # no packed fp32 arithmetic: the compiler forms v_pk_add/mul/fma_f32 from ordinary float code, and
+    # some of their forms have given wrong results on this hardware
     flags = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-munsafe-fp-atomics",
-             "-Wno-unused-result", "-I", str(CSRC / "kernels")] + (["-DPTG_CHECKED"] if checked else [])
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-result", "-I", str(CSRC / "kernels")] + (["-DPTG_CHECKED"] if checked else [])
     flags += [f"-D{d}" for d in defines]
     if not force and out_lib.exists() and srcs and \
             out_lib.stat().st_mtime >= max(_newest_dep(s, headers) for s in srcs):
