@@ -36,6 +36,15 @@ def hip(name: str, *args) -> None:
     _native.call(name, *args, stream_handle())
 
 
+def hip_on(device: torch.device, name: str, *args) -> None:
+    """:func:`hip` on the current stream of ``device``, which need not be the current device."""
+    if _CUR_DEVICE is not None and device.index == _CUR_DEVICE():
+        _native.call(name, *args, stream_handle())
+        return
+    with torch.cuda.device(device):
+        _native.call(name, *args, stream_handle())
+
+
 def need(t: torch.Tensor, dtype: torch.dtype, name: str) -> None:
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")

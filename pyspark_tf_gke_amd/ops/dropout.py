@@ -1,0 +1,159 @@
+"""Dropout drawn from a counter-based generator (csrc/kernels/dropout.hip, rng.h).
+
+The mask is a pure function of ``(seed, step, element index)`` and is never stored: the backward pass
+draws it again.  Element ``i`` of the mask takes the ``i & 7``-th 16-bit piece of Philox4x32-10
+(Salmon et al., SC11) at counter ``(i >> 3, step)`` under the 64-bit ``seed``; it is dropped when the
+piece is below ``round(rate * 65536)``, so the rate is exact to 2**-17, and what is kept is scaled by
+the inverse of that exact keep probability.  Dropped elements are 0 whatever the input holds.
+
+``step`` is a host integer or a one-element int64 device tensor that the kernel reads (a captured HIP
+graph then draws another mask every replay, see :func:`drop_advance`).
+
+``noise_shape`` (Keras): the shape of the mask, 1 (or None) on ONE run of axes that share an entry,
+e.g. ``(N, 1, 1, C)`` or ``(N, 1)``; None draws an entry per element.  GPU tensors run the kernel, CPU
+tensors the reference below.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+
+from ._util import hip_on, on_device, ptr
+
+_M64 = (1 << 64) - 1
+
+
+class Drop(NamedTuple):
+    """A dropout inside a fused operator: rate, 64-bit seed, step (int or int64 device tensor)."""
+
+    rate: float
+    seed: int
+    step: object = 0
+
+
+def threshold(rate: float) -> tuple[int, float]:
+    """(threshold of the 16-bit pieces, scale of what is kept)."""
+    rate = float(rate)
+    if not 0.0 <= rate <= 1.0:  # also refuses NaN
+        raise ValueError(f"dropout: rate must lie in [0, 1], got {rate}")
+    thr = int(round(rate * 65536))
+    return thr, 65536.0 / (65536 - thr) if thr < 65536 else 0.0
+
+
+def _signed(v: int) -> int:
+    v = int(v) & _M64
+    return v - (1 << 64) if v >> 63 else v
+
+
+def step_args(step, device) -> tuple:
+    """(host step, device step tensor or None), checked."""
+    if isinstance(step, torch.Tensor):
+        if step.dtype != torch.int64 or step.numel() != 1:
+            raise TypeError("dropout: a step tensor must hold one int64")
+        if step.device != device:
+            raise ValueError(f"dropout: step lives on {step.device}, the data on {device}")
+        return 0, step
+    return _signed(step), None
+
+
+def mix_seed(seed: int, stream: int) -> int:
+    """A 64-bit seed of its own for each (seed, stream): the SplitMix64 finaliser (Steele, Lea, Flood,
+    OOPSLA 2014) over seed + (stream + 1) * golden ratio."""
+    z = (int(seed) + (int(stream) + 1) * 0x9E3779B97F4A7C15) & _M64
+    z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & _M64
+    z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & _M64
+    return z ^ (z >> 31)
+
+
+def noise_dims(shape, noise_shape) -> tuple[int, int, int]:
+    """(outer, mid, inner) of ``shape`` whose mask is shared over mid."""
+    shape = tuple(int(s) for s in shape)
+    n = math.prod(shape)
+    if noise_shape is None:
+        return n, 1, 1
+    noise = tuple(s if v is None else int(v) for v, s in zip(noise_shape, shape))
+    if len(noise_shape) != len(shape) or any(v not in (1, s) for v, s in zip(noise, shape)):
+        raise ValueError(f"dropout: noise_shape {tuple(noise_shape)} does not broadcast to {shape}")
+    shared = [k for k, (v, s) in enumerate(zip(noise, shape)) if v == 1 and s > 1]
+    if not shared:
+        return n, 1, 1
+    lo, hi = shared[0], shared[-1] + 1
+    if any(noise[k] != 1 for k in range(lo, hi)):
+        raise NotImplementedError(f"dropout: noise_shape {noise} shares two separate runs of axes of {shape}")
+    return math.prod(shape[:lo]), math.prod(shape[lo:hi]), math.prod(shape[hi:])
+
+
+def _pieces(blocks, step: int, seed: int):
+    """[len(blocks), 8] 16-bit pieces (int64): the host reference of rng.h."""
+    lo = 0xFFFFFFFF
+    step &= _M64
+    seed &= _M64
+    c0, c1 = blocks & lo, (blocks >> 32) & lo
+    c2 = torch.full_like(blocks, step & lo)
+    c3 = torch.full_like(blocks, step >> 32)
+    k0, k1 = seed & lo, seed >> 32
+    for _ in range(10):
+        p0, p1 = c0 * 0xD2511F53, c2 * 0xCD9E8D57  # wraps; the masks below read the right bits
+        c0, c1, c2, c3 = (((p1 >> 32) & lo) ^ c1 ^ k0, p1 & lo, ((p0 >> 32) & lo) ^ c3 ^ k1, p0 & lo)
+        k0, k1 = (k0 + 0x9E3779B9) & lo, (k1 + 0xBB67AE85) & lo
+    w = torch.stack((c0, c1, c2, c3), 1)
+    return torch.stack((w & 0xFFFF, w >> 16), 2).reshape(len(blocks), 8)
+
+
+def keep_mask(shape, rate: float, seed: int, step, noise_shape=None) -> torch.Tensor:
+    """The bool mask (host reference), of ``shape``."""
+    thr, _ = threshold(rate)
+    outer, mid, inner = noise_dims(shape, noise_shape)
+    n = outer * inner
+    step = int(step)
+    p = _pieces(torch.arange((n + 7) // 8, dtype=torch.int64), step, int(seed)).reshape(-1)[:n]
+    return (p >= thr).view(outer, 1, inner).expand(outer, mid, inner).reshape(tuple(shape))
+
+
+def _run(name, x, rate, seed, step, out, noise_shape):
+    thr, scale = threshold(rate)
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{name}: expected bfloat16 or float32, got {x.dtype}")
+    if out.dtype != x.dtype or out.shape != x.shape or out.device != x.device:
+        raise ValueError(f"{name}: output must match the input's shape, dtype and device")
+    if not x.is_contiguous() or not out.is_contiguous():
+        raise ValueError(f"{name}: tensor must be contiguous")
+    _, mid, inner = noise_dims(x.shape, noise_shape)
+    host, dev = step_args(step, x.device)
+    if not on_device(x):
+        keep = keep_mask(x.shape, rate, seed, step, noise_shape)
+        out.copy_(torch.where(keep, x.float() * scale, 0.0).to(out.dtype))
+        return out
+    if out.data_ptr() != x.data_ptr() and _overlap(x, out):
+        raise ValueError(f"{name}: input and output overlap")
+    hip_on(x.device, "ptg_dropout", ptr(x), ptr(out), x.numel(), int(x.dtype == torch.float32), thr, scale,
+           _signed(seed), host, ptr(dev), mid, inner)
+    return out
+
+
+def _overlap(a, b) -> bool:
+    size = a.numel() * a.element_size()
+    return a.data_ptr() < b.data_ptr() + size and b.data_ptr() < a.data_ptr() + size
+
+
+def dropout_fwd(x, rate: float, seed: int, step, out, noise_shape=None):
+    """out = keep ? x * scale : 0, bf16 or fp32, ``out`` may be ``x``."""
+    return _run("dropout_fwd", x, rate, seed, step, out, noise_shape)
+
+
+def dropout_bwd(dy, rate: float, seed: int, step, dx, noise_shape=None):
+    """dx = keep ? dy * scale : 0 with the mask of the forward call of the same seed, step and shape."""
+    return _run("dropout_bwd", dy, rate, seed, step, dx, noise_shape)
+
+
+def drop_advance(step):
+    """step += 1 for a device-resident step (a kernel, so a captured graph advances it every replay)."""
+    if step.dtype != torch.int64 or step.numel() != 1:
+        raise TypeError("drop_advance: step must hold one int64")
+    if not on_device(step):
+        step += 1
+        return step
+    hip_on(step.device, "ptg_drop_advance", ptr(step))
+    return step
