@@ -27,6 +27,8 @@ struct BlkArgs {
   int C, tpr, slotwise, sub, nvec;
 };
 
+typedef __attribute__((ext_vector_type(4))) unsigned int vu4_t;
+
 // ---- sums over the LPR lanes of a row (every lane gets the sum) --------------------------------
 template <int CTRL>
 PTG_DEV float dpp_add(float v) {
@@ -49,18 +51,35 @@ PTG_DEV float lanes_sum(float v) {
   return v;
 }
 
-// Sums of two values over a row of `tpr` threads.  Rows of several waves meet in LDS; `phase`
-// alternates between two buffers, so one barrier an exchange is enough: a buffer is written again
-// only after the barrier of the exchange in between.
+// Rows of several waves meet in LDS.  `phase` alternates between two buffers, so one barrier an exchange is
+// enough: a buffer is written again only after the barrier of the exchange in between.  Every lane then
+// takes the entry of wave (lane % waves of a row) and the 16 lanes of a DPP row add up, each wave counted
+// 16 / waves times: no loop over the waves.
 struct RowX {
   float2* lds;  // [2][NT / 64]
   int phase, w, nw, w0, wper;  // wave, waves of the workgroup, first wave of this row, waves of a row
-  PTG_DEV float2* put(float2 v) {
+  float invC, inv_cw;          // 1 / C; 1 / columns of this wave (of the row for LPR < 64)
+  float rep, nk;               // waves of a row / 16; that times the columns of wave (lane % wper)
+  PTG_DEV void init(float2* buf, int tid, int nt, int lpr, int tpr, int C) {
+    lds = buf;
+    phase = 0;
+    w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    nw = nt / 64;
+    wper = tpr >> 6;
+    w0 = lpr < 64 ? 0 : __builtin_amdgcn_readfirstlane((tid / tpr) * wper);
+    const bool multi = lpr == 64 && wper > 1;
+    const int n = multi ? min(max(C - (w - w0) * 512, 0), 512) : C;
+    invC = 1.f / (float)C;
+    inv_cw = n > 0 ? 1.f / (float)n : 0.f;
+    rep = (float)wper * 0.0625f;
+    nk = multi ? (float)min(max(C - (tid & (wper - 1)) * 512, 0), 512) * rep : 0.f;
+  }
+  PTG_DEV float2 put(float2 v) {
     float2* buf = lds + (phase & 1) * nw;
     ++phase;
     if ((threadIdx.x & 63) == 0) buf[w] = v;
     __syncthreads();
-    return buf + w0;
+    return buf[w0 + (threadIdx.x & (wper - 1))];
   }
 };
 template <int LPR>
@@ -68,62 +87,56 @@ PTG_DEV float2 row_sum2(float2 v, RowX& rx) {
   v.x = lanes_sum<LPR>(v.x);
   v.y = lanes_sum<LPR>(v.y);
   if (LPR == 64 && rx.wper > 1) {
-    const float2* p = rx.put(v);
-    v = make_float2(0.f, 0.f);
-    for (int k = 0; k < rx.wper; ++k) { v.x += p[k].x; v.y += p[k].y; }
+    v = rx.put(v);
+    v.x = lanes_sum<16>(v.x * rx.rep);
+    v.y = lanes_sum<16>(v.y * rx.rep);
   }
   return v;
 }
 
-// Mean and 1/std of a row held 8 values a thread (`nv` of them real, the others 0).  LayerNorm takes
-// the squared deviations from each wave's own mean and joins the waves by
+// Mean and 1/std of a row held 8 values a thread (`nv` of them real, the others 0).  The squared
+// deviations are taken from each wave's own mean and joined by
 //   M2 = sum_w M2_w + n_w * (mean_w - mean)^2
-// so no sum of squares around zero cancels, whatever the row's offset; one exchange either way.
-template <int LPR>
-PTG_DEV void row_stats(const float* f, int nv, int C, int kind, float eps, RowX& rx, float& mean, float& rstd) {
+// so no sum of squares around zero cancels, whatever the row's offset; one exchange.  An RMSNorm (layer ==
+// 0) is the same with every mean 0.
+template <int LPR, bool ALN>
+PTG_DEV void row_stats(const float* f, int nv, float layer, float eps, RowX& rx, float& mean, float& rstd) {
   float s = 0.f, q = 0.f;
-  if (kind == NORM_RMS) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q = fmaf(f[j], f[j], q);
-    mean = 0.f;
-    rstd = rsqrtf(row_sum2<LPR>(make_float2(0.f, q), rx).y / (float)C + eps);
-    return;
-  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) s += f[j];
-  s = lanes_sum<LPR>(s);
-  const bool multi = LPR == 64 && rx.wper > 1;
-  const int cw = multi ? min(max(C - (rx.w - rx.w0) * 512, 0), 512) : C;
-  float m = cw > 0 ? s / (float)cw : 0.f;
+  float m = lanes_sum<LPR>(s) * (rx.inv_cw * layer);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float e = f[j] - m;
-    q = j < nv ? fmaf(e, e, q) : q;
+    q = ALN || j < nv ? fmaf(e, e, q) : q;
   }
-  q = lanes_sum<LPR>(q);
-  if (multi) {
-    const float2* p = rx.put(make_float2(m, q));
-    m = 0.f;
-    for (int k = 0; k < rx.wper; ++k) m = fmaf((float)min(max(C - k * 512, 0), 512), p[k].x, m);
-    m /= (float)C;
-    q = 0.f;
-    for (int k = 0; k < rx.wper; ++k) {
-      const float e = p[k].x - m;
-      q += p[k].y + (float)min(max(C - k * 512, 0), 512) * e * e;
-    }
+  q = lanes_sum<LPR>(!ALN || nv ? q : 0.f);
+  if (LPR == 64 && rx.wper > 1) {
+    // a wave's own mean is rounded; the identity above holds for any value near it
+    const float2 p = rx.put(make_float2(m, q));
+    m = lanes_sum<16>(p.x * rx.nk) * rx.invC;
+    const float e = p.x - m;
+    q = lanes_sum<16>(fmaf(rx.nk * e, e, p.y * rx.rep));
   }
   mean = m;
-  rstd = rsqrtf(q / (float)C + eps);
+  rstd = rsqrtf(q * rx.invC + eps);
 }
 
 // ---- 8 consecutive values of a row ---------------------------------------------------------------
-// ALN: 16-byte aligned and always whole.  Otherwise whole groups use unaligned vector accesses and the
-// last group of a row goes value by value.
+// Aligned rows (ALN: 16-byte aligned, C % 8 == 0) go through buffer descriptors that stand at the
+// workgroup's current rows: a lane's offset never changes, rows and columns that do not exist read 0 and
+// are not written, and so does a tensor that is not there (0 bytes): no branch, no 64-bit arithmetic a
+// lane.  Otherwise whole groups use unaligned vector accesses and the last group of a row goes value by
+// value.
 template <typename T> struct Raw8;
 template <> struct Raw8<bf16_t> {
   U4 v;
   PTG_DEV void get(float* f) const { unpack8(v, f); }
   PTG_DEV void set(const float* f) { v = pack8(f); }
+  PTG_DEV void load(Rsrc r, uint32_t off) { v = bload16(r, off); }
+  PTG_DEV void store(Rsrc r, uint32_t off) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(vu4_t, v), r, off, 0, 0);
+  }
 };
 template <> struct Raw8<float> {
   float v[8];
@@ -135,75 +148,179 @@ template <> struct Raw8<float> {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = f[j];
   }
+  PTG_DEV void load(Rsrc r, uint32_t off) {
+    const U4 a = bload16(r, off), b = bload16(r, off + 16);
+    __builtin_memcpy(v, &a, 16);
+    __builtin_memcpy(v + 4, &b, 16);
+  }
+  PTG_DEV void store(Rsrc r, uint32_t off) const {
+    vu4_t a, b;
+    __builtin_memcpy(&a, v, 16);
+    __builtin_memcpy(&b, v + 4, 16);
+    __builtin_amdgcn_raw_buffer_store_b128(a, r, off, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(b, r, off + 16, 0, 0);
+  }
 };
-template <bool ALN, typename T>
-PTG_DEV void load8(Raw8<T>& r, const void* base, long row, int C, int c0, int nv) {
-  const T* p = (const T*)base + row * C + c0;
-  if (ALN) {
-    __builtin_memcpy(&r.v, __builtin_assume_aligned(p, 16), sizeof(r.v));
-  } else if (nv == 8) {
-    __builtin_memcpy(&r.v, p, sizeof(r.v));
-  } else {
+// Where a lane stands: columns c0.. of the row `lag` rows behind the workgroup's base row.
+template <typename T, bool ALN>
+struct Lane {
+  int nv;        // real values of its 8
+  uint32_t off;  // elements from the base row's start
+  uint32_t boff, soff;  // bytes for the descriptors: values, and a float of the row
+  PTG_DEV Lane(int lag, int c0, int C) {
+    nv = ALN ? (c0 < C ? 8 : 0) : min(max(C - c0, 0), 8);
+    off = (uint32_t)lag * C + c0;
+    boff = nv ? off * (uint32_t)sizeof(T) : PTG_OOB;
+    soff = nv ? (uint32_t)lag * 4 : PTG_OOB;
+  }
+  // rows: how many rows from the base row on exist (at most as far as the lanes reach)
+  PTG_DEV static Rsrc rsrc(const void* p, long at, uint32_t rows, int C) {
+    return make_rsrc((const T*)p + at, p ? rows * (uint32_t)C * (uint32_t)sizeof(T) : 0u);
+  }
+  PTG_DEV void load(Raw8<T>& r, const void* base, long at, uint32_t rows, int C, bool on) const {
+    if (ALN) {
+      r.load(rsrc(base, at, rows, C), boff);
+      return;
+    }
     T t[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = j < nv ? p[j] : (T)0;
-    __builtin_memcpy(&r.v, t, sizeof(r.v));
-  }
-}
-template <bool ALN, typename T>
-PTG_DEV void store8(const Raw8<T>& r, void* base, long row, int C, int c0, int nv) {
-  T* p = (T*)base + row * C + c0;
-  if (ALN) {
-    __builtin_memcpy(__builtin_assume_aligned(p, 16), &r.v, sizeof(r.v));
-  } else if (nv == 8) {
-    __builtin_memcpy(p, &r.v, sizeof(r.v));
-  } else {
-    T t[8];
-    __builtin_memcpy(t, &r.v, sizeof(r.v));
+    for (int j = 0; j < 8; ++j) t[j] = (T)0;
+    if (on && base) {
+      const T* p = (const T*)base + at + off;
+      if (nv == 8) {
+        __builtin_memcpy(t, p, sizeof(t));
+      } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < nv) p[j] = t[j];
+        for (int j = 0; j < 8; ++j)
+          if (j < nv) t[j] = p[j];
+      }
+    }
+    __builtin_memcpy(&r.v, t, sizeof(t));
   }
-}
-PTG_DEV void vec8(float* f, const float* p, int c0, int nv, float dflt) {
+  PTG_DEV void store(const Raw8<T>& r, void* base, long at, uint32_t rows, int C, bool on) const {
+    if (ALN) {
+      r.store(rsrc(base, at, rows, C), boff);
+    } else if (on && base) {
+      T* p = (T*)base + at + off;
+      if (nv == 8) {
+        __builtin_memcpy(p, &r.v, sizeof(r.v));
+      } else {
+        T t[8];
+        __builtin_memcpy(t, &r.v, sizeof(r.v));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = p && j < nv ? p[c0 + j] : dflt;
-}
+        for (int j = 0; j < 8; ++j)
+          if (j < nv) p[j] = t[j];
+      }
+    }
+  }
+};
+
+// Column vectors (affine parameters, a gate row).  Rows of up to 2048 columns hold those that are there
+// in LDS (dynamic, [vector][2][C/2 rounded up]), as two planes of 4 values a thread so that a wave reads 16
+// bytes a lane without bank conflicts: in registers they would cost up to 40 of the 128 that leave four
+// waves a SIMD.  Wider rows (NT = 1024) read them from L2.
+struct ColVec {
+  const float* src;  // null: dflt everywhere
+  float dflt;
+};
+template <int NT, int N>
+struct ColVecs {
+  static constexpr bool LDS = NT <= 512;
+  ColVec v[N];
+  int half;
+  // All vectors' loads are issued before the first store: one trip to memory, not one for each.
+  PTG_DEV void init(float* lds, int C, int tid) {
+    half = ((C + 7) & ~7) >> 1;
+    if (!LDS) return;
+    for (int c = tid * 4; c < 2 * half; c += NT * 4) {
+      float4 t[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        t[k] = make_float4(v[k].dflt, v[k].dflt, v[k].dflt, v[k].dflt);
+        if (!v[k].src) continue;
+        if (c + 4 <= C) {
+          __builtin_memcpy(&t[k], v[k].src + c, 16);
+        } else {
+          float e[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) e[j] = c + j < C ? v[k].src[c + j] : v[k].dflt;
+          t[k] = make_float4(e[0], e[1], e[2], e[3]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < N; ++k) *(float4*)(lds + 2 * k * half + ((c >> 2) & 1) * half + (c >> 3) * 4) = t[k];
+    }
+  }
+  // c0 of a lane without columns: any that exist
+  PTG_DEV void get(const float* lds, int k, float* f, int c0, int nv) const {
+    if (LDS) {
+      const float* p = lds + 2 * k * half + (c0 >> 1);
+      const float4 a = *(const float4*)p, b = *(const float4*)(p + half);
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else if (v[k].src && nv == 8) {
+      __builtin_memcpy(f, v[k].src + c0, 32);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = v[k].src && j < nv ? v[k].src[c0 + j] : v[k].dflt;
+    }
+  }
+};
+static inline int col_vec_bytes(int nt, int C, int n) { return nt <= 512 ? n * ((C + 7) & ~7) * 4 : 0; }
 
 template <bool ALN>
-PTG_DEV uint32_t row_keep(const BlkArgs& a, uint64_t step, long row, int c0) {
-  const uint64_t i = (uint64_t)row * (uint64_t)a.C + (uint64_t)c0;
-  return ALN ? keep8(philox(i >> 3, step, a.d.seed), a.d.thr) : keep8_at(i, step, a.d);
+PTG_DEV void row_keep(const BlkArgs& a, uint64_t step, long at, uint32_t off, bool* k) {
+  if (ALN) {
+    keep8(philox(((uint64_t)at >> 3) + (off >> 3), step, a.d.seed), a.d.thr, k);
+  } else {
+    const uint32_t b = keep8_at((uint64_t)at + off, step, a.d);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k[j] = (b >> j) & 1u;
+  }
 }
 
 // ---- rows of a workgroup -------------------------------------------------------------------------
-// A work item is a bundle of row groups, one for each slot (`slotwise`, groups of rpg rows; rpg = 1
-// unless the gate has a row per group), or a part of one long group whose rows the slots share.
+// A work item is a bundle of rows, one for each slot; where the gate has a row per group (GG) a bundle of
+// whole groups, one for each slot (`slotwise`), or a part of one long group whose rows the slots share.
+// A slot stands at row base + lag, base being the same for the workgroup and lag never changing.
+template <bool GG>
 struct RowIter {
-  long item;
+  long item, base, rem;  // rem: rows from base on that exist (slots with lag < rem have a row)
+  long g;                // group of the item (slotwise: of slot 0)
   int j, jn;
-  long g, r0, r1;
-  PTG_DEV void enter(const BlkArgs& a, int slot, int slots) {
+  PTG_DEV static int lag(const BlkArgs& a, int slot) { return GG && a.slotwise ? slot * (int)a.rpg : slot; }
+  // rows that the descriptors cover: as far as the last slot
+  PTG_DEV uint32_t rows(const BlkArgs& a, int slots) const {
+    const long reach = GG && a.slotwise ? (slots - 1) * a.rpg + 1 : slots;
+    return (uint32_t)(rem < reach ? (rem > 0 ? rem : 0) : reach);
+  }
+  PTG_DEV void enter(const BlkArgs& a, int slots) {
     j = 0;
-    if (a.slotwise) {
-      g = item * slots + slot;
-      r0 = g * a.rpg;
-      r1 = item < a.items && r0 < a.M ? r0 + a.rpg : r0;
+    if (!GG) {
+      base = item * slots;
+      rem = a.M - base;
+      g = 0;
+      jn = 1;
+    } else if (a.slotwise) {
+      g = item * slots;
+      base = g * a.rpg;
+      rem = a.M - base;
       jn = (int)a.rpg;
     } else {
       g = item / a.sub;
-      const long len = (a.rpg + a.sub - 1) / a.sub, k = item - g * a.sub;
-      r0 = g * a.rpg + k * len + slot;
-      r1 = item < a.items ? min(g * a.rpg + (k + 1) * len, (g + 1) * a.rpg) : r0;
+      const long len = (a.rpg + a.sub - 1) / a.sub, k = (item - g * a.sub) * len;
+      base = g * a.rpg + k;
+      rem = item < a.items ? min(len, a.rpg - k) : 0;
       jn = (int)((len + slots - 1) / slots);
     }
   }
-  PTG_DEV long row(const BlkArgs& a, int slots) const { return r0 + (a.slotwise ? (long)j : (long)j * slots); }
-  PTG_DEV bool valid(const BlkArgs& a, int slots) const { return row(a, slots) < r1; }
-  PTG_DEV void next(const BlkArgs& a, int slot, int slots) {
-    if (++j >= jn) {
+  PTG_DEV void next(const BlkArgs& a, int slots) {
+    if (GG && ++j < jn) {
+      base += a.slotwise ? 1 : slots;
+      rem -= a.slotwise ? 0 : slots;
+    } else {
       item += gridDim.x;
-      enter(a, slot, slots);
+      enter(a, slots);
     }
   }
 };

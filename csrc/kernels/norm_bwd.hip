@@ -7,8 +7,12 @@
 // h and post(x) are computed again from x and res (and the mask drawn again), in fp32: the pass reads
 // du, dh, x, res and writes dx, dres, each once, and h need not be kept.  Column sums stay in registers
 // over all rows of a workgroup, are joined over its rows in LDS, and a second kernel adds the
-// workgroups' partial sums in a fixed order: no atomics, the same bits every run.
+// workgroups' partial sums in a fixed order: no atomics, the same bits every run.  As in the forward pass
+// the next row's loads are in flight while a row is worked on.
 #include "norm.h"
+#ifndef BWD_OCC
+#define BWD_OCC 2
+#endif
 
 // Joins a thread's column sums over the rows (slots) of the workgroup and writes dst[0..C).
 template <int LPR, int NT, typename D>
@@ -42,117 +46,166 @@ PTG_DEV void flush_cols(float* acc, float* lds, int tid, int tpr, int C, D* dst)
   }
 }
 
-template <typename T, int LPR, int NT, bool ALN, bool PO, bool PR>
-__global__ __launch_bounds__(NT) void block_norm_bwd_k(BlkArgs a) {
-  __shared__ float2 xch[2 * (NT / 64)];
-  __shared__ float cols[NT * 8];
-  const int tid = threadIdx.x, tpr = LPR < 64 ? LPR : a.tpr, slots = NT / tpr, slot = tid / tpr;
-  const int c0 = (tid % tpr) * 8, C = a.C, nv = ALN ? (c0 < C ? 8 : 0) : min(max(C - c0, 0), 8);
-  RowX rx{xch, 0, tid >> 6, NT / 64, LPR < 64 ? 0 : (slot * tpr) >> 6, tpr >> 6};
-  const uint64_t step = a.drop ? drop_step(a.d) : 0;
-  const float invC = 1.f / (float)C;
-  float g1[8], b1[8], g2[8], gt[8];
-  float ag1[8], ab1[8], ag2[8], ab2[8], agt[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) { ag1[j] = 0.f; ab1[j] = 0.f; ag2[j] = 0.f; ab2[j] = 0.f; agt[j] = 0.f; }
+template <typename T>
+struct RowIn {  // a row on its way in
+  Raw8<T> x, r, gu, gh;
+  float m1, s1, m2, s2;
+};
+template <bool ALN, bool PO, bool PR, typename T>
+PTG_DEV void load_row(RowIn<T>& in, const BlkArgs& a, const Lane<T, ALN>& ln, long base, uint32_t rows, bool on) {
+  const long at = base * a.C;
+  ln.load(in.x, a.x, at, rows, a.C, on);
+  if (PR) ln.load(in.r, a.res, at, rows, a.C, on);
+  if (PR) ln.load(in.gu, a.du, at, rows, a.C, on);
+  ln.load(in.gh, a.dh, at, rows, a.C, on);
+  // a row that does not exist, and a lane without columns, take 0 for 1/std: nothing of theirs counts
+  auto stat = [&](int k) {
+    return __uint_as_float(bload4(make_rsrc(a.stats + k * a.M + base, rows * 4), ln.soff));
+  };
   if (PO) {
-    vec8(g1, a.g1, c0, nv, 1.f);
-    vec8(b1, a.b1, c0, nv, 0.f);
+    in.m1 = a.kind1 ? stat(0) : 0.f;
+    in.s1 = a.kind1 ? stat(1) : 1.f;
   }
-  if (PR) vec8(g2, a.g2, c0, nv, 1.f);
-  vec8(gt, a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, c0, nv, 1.f);
-  RowIter it;
+  if (PR) {
+    in.m2 = stat(2);
+    in.s2 = stat(3);
+  }
+}
+
+template <typename T, int LPR, int NT, bool ALN, bool PO, bool PR, bool GG, bool DROP>
+__global__ __launch_bounds__(NT, BWD_OCC) void block_norm_bwd_k(BlkArgs a) {
+  __shared__ float2 xch[2 * (NT / 64)];
+  extern __shared__ float4 dyn[];
+  float* vecs = (float*)dyn;  // column vectors, then [NT * 8] of the joins
+  const int tid = threadIdx.x, tpr = LPR < 64 ? LPR : a.tpr, slots = NT / tpr, slot = tid / tpr;
+  const int C = a.C, c0 = (tid % tpr) * 8, lag = RowIter<GG>::lag(a, slot);
+  const Lane<T, ALN> ln(lag, c0, C);
+  const int nv = ln.nv, cc = nv ? c0 : 0;
+  RowX rx;
+  rx.init(xch, tid, NT, LPR, tpr, C);
+  const uint64_t step = DROP ? drop_step(a.d) : 0;
+  RowIn<T> in;
+  RowIter<GG> it;
   it.item = blockIdx.x;
-  it.enter(a, slot, slots);
+  it.enter(a, slots);
+  uint32_t rows = it.rows(a, slots);
+  bool on = lag < (int)rows && nv > 0;
+  load_row<ALN, PO, PR>(in, a, ln, it.base, rows, on);
+  ColVecs<NT, 4> cv;
+  enum { G1, B1, G2, GV };
+  cv.v[G1] = {PO ? a.g1 : nullptr, 1.f};
+  cv.v[B1] = {PO ? a.b1 : nullptr, 0.f};
+  cv.v[G2] = {PR ? a.g2 : nullptr, 1.f};
+  cv.v[GV] = {a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, 1.f};
+  cv.init(vecs, C, tid);
+  float* cols = vecs + (cv.LDS ? 8 * cv.half : 0);
+  float ag1[8], ab1[8], ag2[8], ab2[8], agt[8], gt[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) { ag1[j] = 0.f; ab1[j] = 0.f; ag2[j] = 0.f; ab2[j] = 0.f; agt[j] = 0.f; gt[j] = 1.f; }
+  const float fs = DROP ? a.scale * a.d.scale : a.scale;  // of a kept element
+  // the sums' shares: mean(g) of a LayerNorm only, mean(g * xhat) of a norm only
+  const float p1 = a.kind1 == NORM_LAYER ? rx.invC : 0.f, q1 = a.kind1 ? rx.invC : 0.f;
+  const float p2 = a.kind2 == NORM_LAYER ? rx.invC : 0.f;
+  __syncthreads();
   while (it.item < a.items) {
-    const long row = it.row(a, slots);
-    const bool on = it.valid(a, slots) && nv > 0;
-    float x[8], r[8], gu[8], gh[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { x[j] = 0.f; r[j] = 0.f; gu[j] = 0.f; gh[j] = 0.f; }
-    float m1 = 0.f, s1 = 0.f, m2 = 0.f, s2 = 0.f;
+    asm volatile("" ::: "memory");  // keeps the column vectors in LDS: hoisted, they cost 32 registers
+    const long at = it.base * C, g = it.g, item = it.item;
+    const uint32_t crows = rows;
+    const bool con = on, first = it.j == 0, last = it.j == it.jn - 1;
+    float xh[8], r[8], gu[8], gh[8], n[8], v[8];
+    bool keep[8];
+    in.x.get(xh);
+    if (PR) in.r.get(r);
+    if (PR) in.gu.get(gu);
+    in.gh.get(gh);
+    const float m1 = in.m1, s1 = in.s1, m2 = in.m2, s2 = in.s2;
+    it.next(a, slots);
+    rows = it.item < a.items ? it.rows(a, slots) : 0;
+    on = lag < (int)rows && nv > 0;
+    load_row<ALN, PO, PR>(in, a, ln, it.base, rows, on);
+    if (DROP) row_keep<ALN>(a, step, at, ln.off, keep);
     Raw8<T> t;
-    if (on) {
-      load8<ALN>(t, a.x, row, C, c0, nv);
-      t.get(x);
-      if (PR && a.res) { load8<ALN>(t, a.res, row, C, c0, nv); t.get(r); }
-      if (PR) { load8<ALN>(t, a.du, row, C, c0, nv); t.get(gu); }
-      if (a.dh) { load8<ALN>(t, a.dh, row, C, c0, nv); t.get(gh); }
-      if (a.gate_mode == GATE_GROUP && it.j == 0) { load8<ALN>(t, a.gate, it.g, C, c0, nv); t.get(gt); }
-      if (PO && a.kind1) { m1 = a.stats[row]; s1 = a.stats[a.M + row]; }
-      if (PR) { m2 = a.stats[2 * a.M + row]; s2 = a.stats[3 * a.M + row]; }
+    const Lane<T, false> gl(0, c0, C);
+    if (GG && first) {
+      gl.load(t, a.gate, (g + (a.slotwise ? slot : 0)) * C, 0, C, con);
+      t.get(gt);
     }
-    const uint32_t keep = a.drop && on ? row_keep<ALN>(a, step, row, c0) : 0xFFu;
-    float n[8], xh[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      xh[j] = PO && a.kind1 ? (x[j] - m1) * s1 : x[j];
-      n[j] = PO && a.kind1 ? fmaf(xh[j], g1[j], b1[j]) : x[j];
-    }
-    if (PR) {
-      float h2[8], gg[8], c1 = 0.f, c2 = 0.f;
+    if (PO) {
+      float b[8];
+      cv.get(vecs, G1, v, cc, nv);
+      cv.get(vecs, B1, b, cc, nv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float d = n[j] * gt[j] * a.scale;
-        const float k = a.drop ? ((keep >> j) & 1u ? d * a.d.scale : 0.f) : d;
-        h2[j] = j < nv ? (r[j] + k - m2) * s2 : 0.f;
-        gg[j] = gu[j] * g2[j];
-        c1 += gg[j];
-        c2 = fmaf(gg[j], h2[j], c2);
-        ag2[j] = fmaf(gu[j], h2[j], ag2[j]);
+        xh[j] = (xh[j] - m1) * s1;
+        n[j] = fmaf(xh[j], v[j], b[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n[j] = xh[j];
+    }
+    if (!GG) cv.get(vecs, GV, gt, cc, nv);
+    if (PR) {
+      float c1 = 0.f, c2 = 0.f;
+      cv.get(vecs, G2, v, cc, nv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float k = n[j] * gt[j] * fs;
+        r[j] = (r[j] + (!DROP || keep[j] ? k : 0.f) - m2) * s2;  // xhat of h
+        if (!ALN) r[j] = j < nv ? r[j] : 0.f;
+        ag2[j] = fmaf(gu[j], r[j], ag2[j]);
         ab2[j] += gu[j];
+        gu[j] *= v[j];
+        c1 += gu[j];
+        c2 = fmaf(gu[j], r[j], c2);
       }
       const float2 c = row_sum2<LPR>(make_float2(c1, c2), rx);
-      const float k1 = a.kind2 == NORM_LAYER ? c.x * invC : 0.f, k2 = c.y * invC;
+      const float k1 = c.x * p2, k2 = c.y * rx.invC;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) gh[j] = fmaf(s2, gg[j] - k1 - h2[j] * k2, gh[j]);
+      for (int j = 0; j < 8; ++j) gh[j] = fmaf(s2, gu[j] - fmaf(r[j], k2, k1), gh[j]);
     }
-    if (a.dres && on) {
+    if (a.dres) {
       t.set(gh);
-      store8<ALN>(t, a.dres, row, C, c0, nv);
+      ln.store(t, a.dres, at, crows, C, con);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float dd = (a.drop ? ((keep >> j) & 1u ? gh[j] * a.d.scale : 0.f) : gh[j]) * a.scale;
+      const float dd = !DROP || keep[j] ? gh[j] * fs : 0.f;
       agt[j] = fmaf(dd, n[j], agt[j]);
       gh[j] = dd * gt[j];
     }
-    if (PO && a.kind1) {
-      float gg[8], c1 = 0.f, c2 = 0.f;
+    if (PO) {
+      float c1 = 0.f, c2 = 0.f;
+      cv.get(vecs, G1, v, cc, nv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        gg[j] = j < nv ? gh[j] * g1[j] : 0.f;
-        c1 += gg[j];
-        c2 = fmaf(gg[j], xh[j], c2);
-        if (on) {
-          ag1[j] = fmaf(gh[j], xh[j], ag1[j]);
-          ab1[j] += gh[j];
-        }
+        ag1[j] = fmaf(gh[j], xh[j], ag1[j]);
+        ab1[j] += gh[j];
+        gh[j] *= v[j];
+        if (!ALN) gh[j] = j < nv ? gh[j] : 0.f;
+        c1 += gh[j];
+        c2 = fmaf(gh[j], xh[j], c2);
       }
       const float2 c = row_sum2<LPR>(make_float2(c1, c2), rx);
-      const float k1 = a.kind1 == NORM_LAYER ? c.x * invC : 0.f, k2 = c.y * invC;
+      const float k1 = c.x * p1, k2 = c.y * q1;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) gh[j] = s1 * (gg[j] - k1 - xh[j] * k2);
+      for (int j = 0; j < 8; ++j) gh[j] = s1 * (gh[j] - fmaf(xh[j], k2, k1));
     }
-    if (a.dx && on) {
+    if (a.dx) {
       t.set(gh);
-      store8<ALN>(t, a.dx, row, C, c0, nv);
+      ln.store(t, a.dx, at, crows, C, con);
     }
-    if (a.gate_mode == GATE_GROUP && it.j == it.jn - 1) {
+    if (GG && last) {
       if (a.slotwise) {  // this slot has its whole group: the sums are final
-        if (on) {
-          t.set(agt);
-          store8<ALN>(t, a.dgate, it.g, C, c0, nv);
-        }
+        t.set(agt);
+        gl.store(t, a.dgate, (g + slot) * C, 0, C, con);
       } else if (a.sub > 1) {
-        flush_cols<LPR, NT>(agt, cols, tid, tpr, C, a.gpart + it.item * C);
+        flush_cols<LPR, NT>(agt, cols, tid, tpr, C, a.gpart + item * C);
       } else {
-        flush_cols<LPR, NT>(agt, cols, tid, tpr, C, (T*)a.dgate + it.item * C);
+        flush_cols<LPR, NT>(agt, cols, tid, tpr, C, (T*)a.dgate + item * C);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) agt[j] = 0.f;
     }
-    it.next(a, slot, slots);
   }
   // partial column sums: [vector][workgroup][C], vectors in the order dgamma2, dbeta2, dgamma1,
   // dbeta1, dgate as far as they are there (nvec)
@@ -209,18 +262,20 @@ __global__ __launch_bounds__(256) void gate_sums_k(const float* src, T* dst, lon
 
 namespace {
 
-constexpr int BWD_WGS = 512;  // workgroups of a backward pass at most: rows of its partial sums
+#ifndef BWD_WGS_
+#define BWD_WGS_ 256
+#endif
+constexpr int BWD_WGS = BWD_WGS_;  // workgroups of a backward pass at most: rows of its partial sums
 
 struct Shape { int lpr, nt, tpr; };
 Shape shape_of(int C) {
-  if (C <= 16) return {2, 256, 2};
-  if (C <= 64) return {8, 256, 8};
-  if (C <= 256) return {32, 256, 32};
-  if (C <= 512) return {64, 256, 64};
-  if (C <= 1024) return {64, 256, 128};
-  if (C <= 2048) return {64, 256, 256};
-  if (C <= 4096) return {64, 512, 512};
-  return {64, 1024, 1024};
+  if (C <= 16) return {2, 512, 2};
+  if (C <= 64) return {8, 512, 8};
+  if (C <= 256) return {32, 512, 32};
+  if (C <= 512) return {64, 512, 64};
+  if (C <= 1024) return {64, 512, 128};
+  if (C <= 2048) return {64, 512, 256};
+  return {64, 1024, C <= 4096 ? 512 : 1024};
 }
 // Work items: bundles of `slots` groups while groups are short; a long group is an item of its own, or
 // is split (`sub`) where there are too few groups to fill the workgroups.
@@ -231,7 +286,7 @@ void plan(BlkArgs& a, const Shape& s, int& grid) {
   if (a.slotwise) {
     a.items = (G + slots - 1) / slots;
   } else {
-    const long want = BWD_WGS / (G < BWD_WGS ? G : BWD_WGS), most = a.rpg / (4 * slots);
+    const long want = BWD_WGS / (G < BWD_WGS ? G : BWD_WGS), most = a.rpg / slots;
     a.sub = (int)(want < most ? want : most);
     if (a.sub < 1) a.sub = 1;
     a.items = G * a.sub;
@@ -239,20 +294,31 @@ void plan(BlkArgs& a, const Shape& s, int& grid) {
   grid = (int)(a.items < BWD_WGS ? a.items : BWD_WGS);
 }
 
-template <typename T, bool ALN, bool PO, bool PR>
+template <typename T, bool ALN, bool PO, bool PR, bool GG, bool DROP>
 void bwd_go(const BlkArgs& a, const Shape& s, int grid, hipStream_t st) {
-  if (s.lpr == 2) block_norm_bwd_k<T, 2, 256, ALN, PO, PR><<<grid, 256, 0, st>>>(a);
-  else if (s.lpr == 8) block_norm_bwd_k<T, 8, 256, ALN, PO, PR><<<grid, 256, 0, st>>>(a);
-  else if (s.lpr == 32) block_norm_bwd_k<T, 32, 256, ALN, PO, PR><<<grid, 256, 0, st>>>(a);
-  else if (s.nt == 256) block_norm_bwd_k<T, 64, 256, ALN, PO, PR><<<grid, 256, 0, st>>>(a);
-  else if (s.nt == 512) block_norm_bwd_k<T, 64, 512, ALN, PO, PR><<<grid, 512, 0, st>>>(a);
-  else block_norm_bwd_k<T, 64, 1024, ALN, PO, PR><<<grid, 1024, 0, st>>>(a);
+  const int lds = col_vec_bytes(s.nt, a.C, 4) + s.nt * 8 * 4;
+  if (s.lpr == 2) block_norm_bwd_k<T, 2, 512, ALN, PO, PR, GG, DROP><<<grid, 512, lds, st>>>(a);
+  else if (s.lpr == 8) block_norm_bwd_k<T, 8, 512, ALN, PO, PR, GG, DROP><<<grid, 512, lds, st>>>(a);
+  else if (s.lpr == 32) block_norm_bwd_k<T, 32, 512, ALN, PO, PR, GG, DROP><<<grid, 512, lds, st>>>(a);
+  else if (s.nt == 512) block_norm_bwd_k<T, 64, 512, ALN, PO, PR, GG, DROP><<<grid, 512, lds, st>>>(a);
+  else block_norm_bwd_k<T, 64, 1024, ALN, PO, PR, GG, DROP><<<grid, 1024, lds, st>>>(a);
+}
+// no norm at all: the post-norm kernel, whose kind1 == 0 is the identity
+template <typename T, bool ALN, bool GG, bool DROP>
+void bwd_kind(const BlkArgs& a, const Shape& s, int grid, hipStream_t st) {
+  if (!a.kind2) bwd_go<T, ALN, true, false, GG, DROP>(a, s, grid, st);
+  else if (!a.kind1) bwd_go<T, ALN, false, true, GG, DROP>(a, s, grid, st);
+  else bwd_go<T, ALN, true, true, GG, DROP>(a, s, grid, st);
 }
 template <typename T, bool ALN>
-void bwd_kind(const BlkArgs& a, const Shape& s, int grid, hipStream_t st) {
-  if (!a.kind2) bwd_go<T, ALN, true, false>(a, s, grid, st);
-  else if (!a.kind1) bwd_go<T, ALN, false, true>(a, s, grid, st);
-  else bwd_go<T, ALN, true, true>(a, s, grid, st);
+void bwd_mode(const BlkArgs& a, const Shape& s, int grid, hipStream_t st) {
+  if (a.gate_mode == GATE_GROUP) {
+    if (a.drop) bwd_kind<T, ALN, true, true>(a, s, grid, st);
+    else bwd_kind<T, ALN, true, false>(a, s, grid, st);
+  } else {
+    if (a.drop) bwd_kind<T, ALN, false, true>(a, s, grid, st);
+    else bwd_kind<T, ALN, false, false>(a, s, grid, st);
+  }
 }
 
 }  // namespace
@@ -309,8 +375,8 @@ int ptg_block_norm_bwd(const void* x, const void* res, const void* gate, const v
   a.part = (float*)ws;
   a.gpart = (float*)ws + (long)a.nvec * grid * C;
   cs.src = a.part;
-  if (f32) { if (aligned) bwd_kind<float, true>(a, s, grid, stream); else bwd_kind<float, false>(a, s, grid, stream); }
-  else { if (aligned) bwd_kind<bf16_t, true>(a, s, grid, stream); else bwd_kind<bf16_t, false>(a, s, grid, stream); }
+  if (f32) { if (aligned) bwd_mode<float, true>(a, s, grid, stream); else bwd_mode<float, false>(a, s, grid, stream); }
+  else { if (aligned) bwd_mode<bf16_t, true>(a, s, grid, stream); else bwd_mode<bf16_t, false>(a, s, grid, stream); }
   if (a.nvec) col_sums_k<<<dim3((C + 31) / 32, a.nvec), 1024, 0, stream>>>(cs, grid, C);
   if (gate_mode == GATE_GROUP && a.sub > 1) {
     const long n = (M / rpg) * C;

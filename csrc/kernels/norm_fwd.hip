@@ -1,92 +1,138 @@
 // Block norm, forward (norm.h): d = drop(scale * gate * post(x)); h = res + d; u = pre(h).
 //
 // Bound by HBM: x and res in, h and u out, each once; statistics, the gate, the dropout mask and both
-// affine maps live in registers between the load and the stores of a row.  u is taken from the
-// unrounded h.  Statistics are fp32 and kept for the backward pass ([4][M]).
+// affine maps live in registers between the load and the stores of a row.  The next row's loads are
+// issued before the current row is worked on, so the row sums (and the barrier of rows of several waves)
+// run while memory is busy.  u is taken from the unrounded h.  Statistics are fp32 and kept for the
+// backward pass ([4][M]).
 #include "norm.h"
 
-template <typename T, int LPR, int NT, bool ALN>
+template <typename T, int LPR, int NT, bool ALN, bool PO, bool PR, bool DROP>
 __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
   __shared__ float2 xch[2 * (NT / 64)];
+  extern __shared__ float4 dyn[];
+  float* vecs = (float*)dyn;
   const int tid = threadIdx.x, tpr = LPR < 64 ? LPR : a.tpr, slots = NT / tpr, slot = tid / tpr;
-  const int c0 = (tid % tpr) * 8, C = a.C, nv = ALN ? (c0 < C ? 8 : 0) : min(max(C - c0, 0), 8);
-  RowX rx{xch, 0, tid >> 6, NT / 64, LPR < 64 ? 0 : (slot * tpr) >> 6, tpr >> 6};
-  const uint64_t step = a.drop ? drop_step(a.d) : 0;
-  float g1[8], b1[8], g2[8], b2[8], gt[8];
-  vec8(g1, a.g1, c0, nv, 1.f);
-  vec8(b1, a.b1, c0, nv, 0.f);
-  vec8(g2, a.g2, c0, nv, 1.f);
-  vec8(b2, a.b2, c0, nv, 0.f);
-  vec8(gt, a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, c0, nv, 1.f);
-  for (long r0 = (long)blockIdx.x * slots; r0 < a.M; r0 += (long)gridDim.x * slots) {
-    const long row = r0 + slot;
-    const bool on = row < a.M && nv > 0;
-    Raw8<T> rx8, rr8, rg8;
-    float f[8], r[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { f[j] = 0.f; r[j] = 0.f; }
-    if (on) {
-      load8<ALN>(rx8, a.x, row, C, c0, nv);
-      if (a.res) load8<ALN>(rr8, a.res, row, C, c0, nv);
-      if (a.gate_mode == GATE_GROUP) load8<ALN>(rg8, a.gate, row / a.rpg, C, c0, nv);
-      rx8.get(f);
-      if (a.res) rr8.get(r);
-      if (a.gate_mode == GATE_GROUP) rg8.get(gt);
-    }
+  const int C = a.C, c0 = (tid % tpr) * 8;
+  const Lane<T, ALN> ln(slot, c0, C);
+  const int nv = ln.nv, cc = nv ? c0 : 0;
+  RowX rx;
+  rx.init(xch, tid, NT, LPR, tpr, C);
+  const uint64_t step = DROP ? drop_step(a.d) : 0;
+  ColVecs<NT, 5> cv;
+  enum { G1, B1, G2, B2, GV };
+  long r0 = (long)blockIdx.x * slots;
+  const long stride = (long)gridDim.x * slots;
+  auto rows_at = [&](long r) { return (uint32_t)(a.M - r < slots ? (a.M > r ? a.M - r : 0) : slots); };
+  uint32_t rows = rows_at(r0);
+  bool on = slot < (int)rows && nv > 0;
+  Raw8<T> nx, nr, t;
+  ln.load(nx, a.x, r0 * C, rows, C, on);
+  ln.load(nr, a.res, r0 * C, rows, C, on);
+  cv.v[G1] = {PO ? a.g1 : nullptr, 1.f};
+  cv.v[B1] = {PO ? a.b1 : nullptr, 0.f};
+  cv.v[G2] = {PR ? a.g2 : nullptr, 1.f};
+  cv.v[B2] = {PR ? a.b2 : nullptr, 0.f};
+  cv.v[GV] = {a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, 1.f};
+  cv.init(vecs, C, tid);
+  const float sc = DROP ? a.scale * a.d.scale : a.scale;
+  const float lay1 = a.kind1 == NORM_LAYER ? 1.f : 0.f, lay2 = a.kind2 == NORM_LAYER ? 1.f : 0.f;
+  const bool full = C == tpr * 8;
+  __syncthreads();
+  while (r0 < a.M) {
+    asm volatile("" ::: "memory");  // the column vectors stay in LDS
+    float f[8], r[8], v[8], w[8];
+    nx.get(f);
+    nr.get(r);
+    const long cur = r0, at = r0 * C;
+    const uint32_t crows = rows;
+    const bool con = on;
+    r0 += stride;
+    rows = rows_at(r0);
+    on = slot < (int)rows && nv > 0;
+    ln.load(nx, a.x, r0 * C, rows, C, on);
+    ln.load(nr, a.res, r0 * C, rows, C, on);
     float m1 = 0.f, s1 = 1.f, m2 = 0.f, s2 = 1.f;
-    if (a.kind1) {
-      row_stats<LPR>(f, nv, C, a.kind1, a.eps1, rx, m1, s1);
+    if (PO) {
+      row_stats<LPR, ALN>(f, nv, lay1, a.eps1, rx, m1, s1);
+      cv.get(vecs, G1, v, cc, nv);
+      cv.get(vecs, B1, w, cc, nv);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = fmaf((f[j] - m1) * s1, g1[j], b1[j]);
+      for (int j = 0; j < 8; ++j) f[j] = fmaf((f[j] - m1) * s1, v[j], w[j]);
     }
-    const uint32_t keep = a.drop && on ? row_keep<ALN>(a, step, row, c0) : 0xFFu;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float d = f[j] * gt[j] * a.scale;
-      const float k = a.drop ? ((keep >> j) & 1u ? d * a.d.scale : 0.f) : d;
-      f[j] = j < nv ? r[j] + k : 0.f;
-    }
-    if (a.h && on) {
-      rx8.set(f);
-      store8<ALN>(rx8, a.h, row, C, c0, nv);
-    }
-    if (a.kind2) {
-      row_stats<LPR>(f, nv, C, a.kind2, a.eps2, rx, m2, s2);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = fmaf((f[j] - m2) * s2, g2[j], b2[j]);
-      if (on) {
-        rx8.set(f);
-        store8<ALN>(rx8, a.u, row, C, c0, nv);
+    if (a.gate_mode) {
+      if (a.gate_mode == GATE_VEC) {
+        cv.get(vecs, GV, v, cc, nv);
+      } else if (con) {
+        const Lane<T, false> gl(0, c0, C);
+        gl.load(t, a.gate, (cur + slot) / a.rpg * C, 0, C, true);
+        t.get(v);
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= v[j];
     }
-    if (a.stats && row < a.M && c0 == 0) {
-      a.stats[row] = m1;
-      a.stats[a.M + row] = s1;
-      a.stats[2 * a.M + row] = m2;
-      a.stats[3 * a.M + row] = s2;
+    if (DROP) {
+      bool keep[8];
+      row_keep<ALN>(a, step, at, ln.off, keep);
+      // a dropped value is 0 whatever the branch holds
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = r[j] + (keep[j] ? f[j] * sc : 0.f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = fmaf(f[j], sc, r[j]);
+    }
+    if (!ALN || !full) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = j < nv ? f[j] : 0.f;
+    }
+    if (a.h) {
+      t.set(f);
+      ln.store(t, a.h, at, crows, C, con);
+    }
+    if (PR) {
+      row_stats<LPR, ALN>(f, nv, lay2, a.eps2, rx, m2, s2);
+      cv.get(vecs, G2, v, cc, nv);
+      cv.get(vecs, B2, w, cc, nv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = fmaf((f[j] - m2) * s2, v[j], w[j]);
+      t.set(f);
+      ln.store(t, a.u, at, crows, C, con);
+    }
+    if (a.stats && con && c0 == 0) {
+      float* st = a.stats + cur + slot;
+      st[0] = m1;
+      st[a.M] = s1;
+      st[2 * a.M] = m2;
+      st[3 * a.M] = s2;
     }
   }
 }
 
 namespace {
-template <typename T, bool ALN>
+template <typename T, bool ALN, bool PO, bool PR, bool DROP>
 int fwd_launch(const BlkArgs& a, hipStream_t stream) {
   auto go = [&](auto kern, int nt, int tpr) {
     BlkArgs b = a;
     b.tpr = tpr;
-    const long slots = nt / tpr, wgs = (a.M + slots - 1) / slots, cap = 2048L * 256 / nt;
-    kern<<<(int)(wgs < cap ? wgs : cap), nt, 0, stream>>>(b);
+    const long slots = nt / tpr, wgs = (a.M + slots - 1) / slots, cap = 1024L * 256 / nt;  // four waves a SIMD
+    kern<<<(int)(wgs < cap ? wgs : cap), nt, col_vec_bytes(nt, a.C, 5), stream>>>(b);
   };
   const int C = a.C;
-  if (C <= 16) go(block_norm_fwd_k<T, 2, 256, ALN>, 256, 2);
-  else if (C <= 64) go(block_norm_fwd_k<T, 8, 256, ALN>, 256, 8);
-  else if (C <= 256) go(block_norm_fwd_k<T, 32, 256, ALN>, 256, 32);
-  else if (C <= 512) go(block_norm_fwd_k<T, 64, 256, ALN>, 256, 64);
-  else if (C <= 1024) go(block_norm_fwd_k<T, 64, 256, ALN>, 256, 128);
-  else if (C <= 2048) go(block_norm_fwd_k<T, 64, 256, ALN>, 256, 256);
-  else if (C <= 4096) go(block_norm_fwd_k<T, 64, 512, ALN>, 512, 512);
-  else go(block_norm_fwd_k<T, 64, 1024, ALN>, 1024, 1024);
+  if (C <= 16) go(block_norm_fwd_k<T, 2, 256, ALN, PO, PR, DROP>, 256, 2);
+  else if (C <= 64) go(block_norm_fwd_k<T, 8, 256, ALN, PO, PR, DROP>, 256, 8);
+  else if (C <= 256) go(block_norm_fwd_k<T, 32, 256, ALN, PO, PR, DROP>, 256, 32);
+  else if (C <= 2048) go(block_norm_fwd_k<T, 64, 256, ALN, PO, PR, DROP>, 256, C <= 512 ? 64 : C <= 1024 ? 128 : 256);
+  else go(block_norm_fwd_k<T, 64, 1024, ALN, PO, PR, DROP>, 1024, C <= 4096 ? 512 : 1024);
   PTG_RETURN_LAUNCH();
+}
+template <typename T, bool ALN, bool DROP>
+int fwd_kind(const BlkArgs& a, hipStream_t stream) {
+  if (a.kind1) return a.kind2 ? fwd_launch<T, ALN, true, true, DROP>(a, stream) : fwd_launch<T, ALN, true, false, DROP>(a, stream);
+  return a.kind2 ? fwd_launch<T, ALN, false, true, DROP>(a, stream) : fwd_launch<T, ALN, false, false, DROP>(a, stream);
+}
+template <typename T, bool ALN>
+int fwd_drop(const BlkArgs& a, hipStream_t stream) {
+  return a.drop ? fwd_kind<T, ALN, true>(a, stream) : fwd_kind<T, ALN, false>(a, stream);
 }
 }  // namespace
 
@@ -107,8 +153,8 @@ int ptg_block_norm_fwd(const void* x, const void* res, const void* gate, void* h
   a.M = M; a.C = C; a.kind1 = kind1; a.kind2 = kind2; a.eps1 = eps1; a.eps2 = eps2;
   a.gate_mode = gate_mode; a.rpg = rpg > 0 ? rpg : 1; a.scale = scale; a.drop = drop;
   a.d = drop_args(thr, dscale, seed, step, step_dev);
-  if (f32) return aligned ? fwd_launch<float, true>(a, stream) : fwd_launch<float, false>(a, stream);
-  return aligned ? fwd_launch<bf16_t, true>(a, stream) : fwd_launch<bf16_t, false>(a, stream);
+  if (f32) return aligned ? fwd_drop<float, true>(a, stream) : fwd_drop<float, false>(a, stream);
+  return aligned ? fwd_drop<bf16_t, true>(a, stream) : fwd_drop<bf16_t, false>(a, stream);
 }
 
 }  // extern "C"

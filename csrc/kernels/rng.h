@@ -50,6 +50,15 @@ PTG_DEV uint32_t keep8(const U4& w, uint32_t thr) {
   }
   return b;
 }
+// The same as 8 conditions: each compares a half word in place and lands in a lane mask.
+PTG_DEV void keep8(const U4& w, uint32_t thr, bool* k) {
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    k[2 * j] = (v[j] & 0xFFFFu) >= thr;
+    k[2 * j + 1] = (v[j] >> 16) >= thr;
+  }
+}
 // keep bits of the 8 elements from index i on; only an index that is no multiple of 8 needs the
 // second draw
 PTG_DEV uint32_t keep8_at(uint64_t i, uint64_t step, const DropArgs& d) {

@@ -143,7 +143,8 @@ def int4_dequantize(w: Int4Weight) -> torch.Tensor:
 _WS: dict = {}
 
 
-def _ws_floats(batch: int, w: Int4Weight) -> int:
+def int4_workspace_floats(batch: int, w: Int4Weight) -> int:
+    """Floats of :func:`int4_workspace`."""
     key = (batch, w.n, w.k)
     v = _WS.get(key)
     if v is None:
@@ -162,7 +163,7 @@ def int4_workspace(batch: int, w: Int4Weight) -> torch.Tensor | None:
     same time - on two streams, or in two captured graphs - need one each."""
     if not on_device(w.tiles):
         return None
-    n = _ws_floats(batch, w)
+    n = int4_workspace_floats(batch, w)
     return torch.empty(n, dtype=torch.float32, device=w.tiles.device) if n else None
 
 
@@ -189,7 +190,7 @@ def int4_dense_fwd(x, w: Int4Weight, bias, act, out, workspace=None):
         return out
     if x.dtype != torch.bfloat16:
         raise TypeError(f"int4_dense: x must be bfloat16, got {x.dtype}")
-    need = _ws_floats(B, w)
+    need = int4_workspace_floats(B, w)
     if need and workspace is None:
         workspace = torch.empty(need, dtype=torch.float32, device=dev)
     elif need and (workspace.dtype != torch.float32 or workspace.numel() < need or workspace.device != dev

@@ -68,7 +68,9 @@ def test_constant_rows_and_zero_rows(hip_built):
     x[1] = 3.25
     u = torch.empty_like(x)
     N.block_norm_fwd(x, pre=N.Norm("layer", None, None, 1e-3), u=u)
-    assert not u.any()
+    # the sums of 3.25 are exact; 1 / 640 and the product with it are rounded, so the mean is off by at most
+    # 2 * 2**-24 * 3.25 (3 with second-order terms), seen through 1 / sqrt(epsilon)
+    assert not u[[0, 2, 3]].any() and float(u[1].abs().max()) <= 3 * 2.0**-24 * 3.25 / 1e-3**0.5
     N.block_norm_fwd(x, pre=N.Norm("rms", None, None, 1e-6), u=u)
     assert not u[0].any() and abs(float(u[1, 0]) - 1) < 1e-6
 
