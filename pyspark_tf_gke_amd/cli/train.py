@@ -63,6 +63,8 @@ def parse_args(argv: List[str]):
     head = p.add_mutually_exclusive_group()
     head.add_argument("--flat", dest="flat", action="store_true", default=True)
     head.add_argument("--gap", dest="flat", action="store_false")
+    p.add_argument("--dropout", type=float, default=0.0,
+                   help="share of the features in front of the output head that training drops")
     p.add_argument("--interactive", action="store_true")
     p.add_argument("--plot", action="store_true")
     p.add_argument("--checkpoint-every", type=int, default=0, help="save a resumable checkpoint every N epochs")
@@ -193,7 +195,7 @@ def run_deep_training(data_source: str, output_dir: str, epochs: int, batch_size
             return ds.shuffle(min(3000, len(X)), seed=seed).batch(batch_size).repeat()
 
         with strategy.scope():
-            model = build_deep_model(input_dim, num_classes)
+            model = build_deep_model(input_dim, num_classes, dropout=getattr(args, "dropout", 0.0))
             optimizer = nn.optimizers.Adam(learning_rate=1e-4)
             loss_obj = nn.losses.SparseCategoricalCrossentropy()
             metrics = [nn.metrics.Mean("loss"), nn.metrics.SparseCategoricalAccuracy("accuracy")]
@@ -210,7 +212,7 @@ def run_deep_training(data_source: str, output_dir: str, epochs: int, batch_size
         tr, va = idx[:-val], idx[-val:]
         ctx = strategy.scope() if strategy is not None else _null()
         with ctx:
-            model = build_deep_model(input_dim, num_classes)
+            model = build_deep_model(input_dim, num_classes, dropout=getattr(args, "dropout", 0.0))
         ds_train = Dataset.from_tensor_slices((X[tr], y[tr]))
         if strategy is not None and strategy.world_size > 1:
             ds_train = ds_train.shard(strategy.world_size, strategy.rank)
@@ -253,7 +255,8 @@ def run_image_training(data_dir: str, output_dir: str, epochs: int, batch_size: 
 
         with strategy.scope():
             model = build_cnn_model(shape, num_outputs=2, flat=flat_layer, summary=True,
-                                    print_fn=print if _is_chief() else (lambda *a: None))
+                                    print_fn=print if _is_chief() else (lambda *a: None),
+                                    dropout=getattr(args, "dropout", 0.0))
             optimizer = nn.optimizers.Adam(learning_rate=1e-4)
             loss_obj = nn.losses.MeanSquaredError()
             metrics = [nn.metrics.Mean("loss"), nn.metrics.MeanAbsoluteError("mae"), nn.metrics.MeanSquaredError("mse")]
@@ -279,7 +282,8 @@ def run_image_training(data_dir: str, output_dir: str, epochs: int, batch_size: 
         ctx = strategy.scope() if strategy is not None else _null()
         with ctx:
             model = build_cnn_model(shape, num_outputs=2, flat=flat_layer, summary=True,
-                                    print_fn=print if _is_chief() else (lambda *a: None))
+                                    print_fn=print if _is_chief() else (lambda *a: None),
+                                    dropout=getattr(args, "dropout", 0.0))
         cbs = []
         if args is not None and args.checkpoint_every:
             from ..utils.checkpoint import CheckpointCallback

@@ -17,13 +17,16 @@ from .. import nn
 from ..nn import layers as L
 
 
-def build_deep_model(input_dim: int, num_classes: int, compile: bool = True, device=None) -> nn.Sequential:
+def build_deep_model(input_dim: int, num_classes: int, compile: bool = True, device=None,
+                     dropout: float = 0.0) -> nn.Sequential:
+    """``dropout`` > 0 drops that share of the last hidden layer in training."""
     L.reset_name_counters()
     m = nn.Sequential([
         nn.Input(shape=(input_dim,)),
         nn.Dense(16, activation="relu"),
         nn.Dense(32, activation="relu"),
         nn.Dense(64, activation="relu"),
+        *([nn.Dropout(dropout)] if dropout > 0 else []),
         nn.Dense(num_classes, activation="softmax"),
     ])
     m.build(device=device)
@@ -34,7 +37,8 @@ def build_deep_model(input_dim: int, num_classes: int, compile: bool = True, dev
 
 
 def build_cnn_model(input_shape=(256, 320, 3), num_outputs: int = 2, flat: bool = False, compile: bool = True,
-                    summary: bool = True, print_fn=None, device=None) -> nn.Sequential:
+                    summary: bool = True, print_fn=None, device=None, dropout: float = 0.0) -> nn.Sequential:
+    """``dropout`` > 0 drops that share of the features in front of the Dense head in training."""
     L.reset_name_counters()
     m = nn.Sequential([
         nn.Input(shape=input_shape),
@@ -44,6 +48,7 @@ def build_cnn_model(input_shape=(256, 320, 3), num_outputs: int = 2, flat: bool 
         nn.Conv2D(64, 5, padding="same"), nn.PReLU(), nn.MaxPooling2D(),
         nn.Conv2D(64, 5, padding="same"), nn.PReLU(),
         nn.Flatten() if flat else nn.GlobalAveragePooling2D(),
+        *([nn.Dropout(dropout)] if dropout > 0 else []),
         nn.Dense(2048, activation="relu") if flat else nn.Dense(128, activation="relu"),
         nn.Dense(num_outputs, activation="linear"),
     ])

@@ -9,6 +9,7 @@ Keras layers (:mod:`.layers`) are lowered to device ops that own their forward/b
   for narrow ones (N <= 64: the MLP and the 2-output regression head).  A narrow Dense also
   applies the previous layer's ReLU mask inside its dX kernel.
 * ``FlattenOp`` (a view), ``GAPOp``, ``PReLUOp``/``PoolOp`` (unfused fallbacks).
+* Dropout, row norms, LayerScale and Rescaling: :mod:`.norm_ops`.
 
 Activations live in a :class:`Workspace` keyed by op and shape, so every step reuses the same
 device buffers (stable addresses; capturable into a HIP graph).  Reference: the model builders of
@@ -431,6 +432,24 @@ class DenseOp(Op):
         self.logits_only = False  # softmax folded into the loss
         self.fused_update = None  # optimizers.FusedAdamStep during a fused-update training step
 
+    def _forward_int4(self, x, b, act, ws, training):
+        """Inference on 4-bit weights (layers.Dense.quantize)."""
+        from ..ops import quant as Q
+
+        if training:
+            raise RuntimeError(f"{self.name}: a quantized layer is for inference only")
+        w = self.dense.int4
+        B = x.shape[0]
+        x = _bf16(x, ws, self.name + "/x16").contiguous()
+        wsp = None
+        if x.is_cuda:
+            n = Q.int4_workspace_floats(B, w)
+            wsp = ws.get(self.name + "/int4", (n,), torch.float32, x.device) if n else None
+        soft = act == "softmax"
+        y = ws.get(self.name + "/y4", (B, w.n), torch.float32 if soft else torch.bfloat16, x.device)
+        Q.int4_dense_fwd(x, w, b, None if soft else act, y, workspace=wsp)
+        return torch.softmax(y, -1) if soft else y
+
     def forward(self, x, ws, training):
         x = x.reshape(x.shape[0], -1)
         B = x.shape[0]
@@ -438,6 +457,10 @@ class DenseOp(Op):
         dev = x.device
         b = self.dense.bias.data if self.dense.bias is not None else None
         act = None if (self.logits_only and self.act == "softmax") else self.act
+        if self.dense.int4 is not None:
+            y = self._forward_int4(x, b, act, ws, training)
+            self._x, self._y = x, y
+            return y
         if self.big:
             x = _bf16(x, ws, self.name + "/x16")
             y = ws.get(self.name + "/y", (B, N), torch.bfloat16, dev)
@@ -663,10 +686,25 @@ def lower(layers: list) -> list:
             ops.append(PoolOp(l)); i += 1
         elif isinstance(l, L.ReLU):
             ops.append(ReLUOp(l)); i += 1
+        elif isinstance(l, (L.LayerNormalization, L.RMSNormalization, L.LayerScale, L.Rescaling, L.Dropout)):
+            from . import norm_ops as NO
+
+            chain, j = NO.Chain(), i
+            while j < len(seq) and not isinstance(seq[j], L.Multiply) and chain.take(seq[j]):
+                j += 1
+            if j <= i + 1 and isinstance(l, L.Dropout):
+                ops.append(NO.DropoutOp(l)); j = i + 1
+            else:
+                ops.append(NO.SeqBlockOp(chain.op()))
+            i = j
         else:
             raise NotImplementedError(type(l).__name__)
     if ops:
         ops[0].first = True
+    if any(isinstance(l, L.Dropout) for l in seq):
+        from . import norm_ops as NO
+
+        NO.bind_drop_state(ops)
     for k in range(1, len(ops)):
         ops[k].below = ops[k - 1]
     # ReLU-mask hand-off: a skinny Dense applies the previous relu-Dense's mask in its dX

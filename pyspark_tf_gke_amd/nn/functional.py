@@ -11,6 +11,10 @@ Lowering fuses the DAG into device ops (:mod:`.graph_ops`):
   applies the ReLU.  The residual ``Add`` is fused into whichever branch is computed *last*, so the
   other branch is already available.
 * ``ZeroPadding2D`` is folded into the padding of the following conv or max-pool.
+* ``[norm] -> [LayerScale | Multiply] -> [Rescaling] -> [Dropout] -> Add -> [norm]`` (norm:
+  LayerNormalization or RMSNormalization) becomes ONE :class:`~.norm_ops.BlockOp` with two outputs, the
+  stream and its normalised form.  The ``Add`` and a ``Multiply`` are fused where their other input is
+  already there.
 * everything else maps to the Sequential engine's ops (Dense, GAP, Flatten, PReLU...) or generic
   BN / Add / ReLU / MaxPool ops.
 
@@ -23,10 +27,12 @@ from __future__ import annotations
 import time
 
 import numpy as np
+import torch
 
 from . import engine as E
 from . import graph_ops as G
 from . import layers as L
+from . import norm_ops as NO
 from .model import Sequential
 from .params import ParamStore
 from .. import config
@@ -80,29 +86,52 @@ class GraphPlan:
         for op in self.ops:
             if pre_op is not None:
                 pre_op(op)
-            vals[op.output] = op.forward([vals[i] for i in op.inputs], ws, training)
+            res = op.forward([vals[i] for i in op.inputs], ws, training)
+            outs = getattr(op, "outputs", None)
+            if outs is None:
+                vals[op.output] = res
+            else:
+                vals.update(zip(outs, res))
         return vals[self.output_idx]
 
     def backward(self, dy, ws, on_op_done=None):
-        from ..ops import bn as KB
-
         grads = {self.output_idx: dy}
         for op in reversed(self.ops):
-            g = grads.pop(op.output, None)
-            if g is None:
-                continue
+            outs = getattr(op, "outputs", None)
+            if outs is None:
+                g = grads.pop(op.output, None)
+                if g is None:
+                    continue
+            else:
+                g = [grads.pop(o, None) for o in outs]
+                if all(t is None for t in g):
+                    continue
             existing = [grads.get(i) for i in op.inputs]
             res = op.backward(g, ws, existing)
-            for i, gi, ex in zip(op.inputs, res, existing):
+            for i, gi in zip(op.inputs, res):
                 if gi is None or i == self.input_idx:
                     continue
+                ex = grads.get(i)  # also what this op's other input, the same tensor, gave just now
                 if ex is None:
                     grads[i] = gi
                 elif gi is not ex:
-                    KB.add_(ex, gi, ex)
+                    _add_into(ex, gi)
             if on_op_done is not None:
                 on_op_done(op)
         return grads.get(self.input_idx)
+
+
+def _add_into(ex, g) -> None:
+    """ex += g (either bf16 or fp32, the result in ex's type)."""
+    from ..ops import bn as KB
+    from ..ops import norm as NM
+
+    g = g.reshape(ex.shape)
+    if ex.dtype == g.dtype == torch.bfloat16:
+        KB.add_(ex, g, ex)
+    else:
+        NM.block_norm_fwd(g.to(ex.dtype).view(-1, g.shape[-1]), res=ex.view(-1, g.shape[-1]),
+                          h=ex.view(-1, g.shape[-1]))
 
 
 def _lower(nodes: list, input_idx: int) -> list:
@@ -121,6 +150,7 @@ def _lower(nodes: list, input_idx: int) -> list:
     alias: dict = {}  # folded node -> tensor id it forwards
     pad_of: dict = {}  # conv/pool node -> extra zero padding folded from a ZeroPadding2D producer
     claimed: set = set()
+    later: dict = {}  # node -> op that starts at an earlier node and runs here
     ops = []
 
     def src(k):
@@ -128,7 +158,65 @@ def _lower(nodes: list, input_idx: int) -> list:
             k = alias[k]
         return k
 
+    def norm_of(k):
+        """The first row norm that reads tensor k (it joins the op that writes k), or None."""
+        for c in consumers[k]:
+            if c not in claimed and NO.is_norm(nodes[c].layer):
+                return c
+        return None
+
+    def close(chain, k, x, res, add_k):
+        """The BlockOp of a chain that ends in tensor k: its inputs x + [res], the norm behind an Add."""
+        pre_k = norm_of(k) if add_k is not None else None
+        if pre_k is not None:
+            claimed.add(pre_k)
+        want_h = pre_k is None or len(consumers[k]) > 1
+        op = chain.op(res is not None, nodes[pre_k].layer if pre_k is not None else None, want_h)
+        outs = ([k] if op.want_h else []) + ([pre_k] if pre_k is not None else [])
+        return NO.BlockNode(op, x + ([res] if res is not None else []), outs or [k])
+
+    def block_boundary(k, ins):
+        """Lower the chain that starts at node k (a norm, LayerScale, Multiply, Rescaling or Dropout):
+        (node that it runs at, op).  With a gate that is where the Multiply stands: the gate may be
+        computed between k and there."""
+        chain, end, x = NO.Chain(), k, [src(ins[0])]
+        nxt, gate_k, at = k, None, k
+        while nxt is not None and nxt not in claimed:
+            lay = nodes[nxt].layer
+            others = [idx[id(i)] for i in nodes[nxt].inputs]
+            if isinstance(lay, L.Multiply):
+                if nxt != k and (others[0] != end or others[1] == end):
+                    break
+                if not chain.take(lay):
+                    break
+                gate_k, at = others[1], nxt
+            elif not chain.take(lay):
+                break
+            if nxt != k:
+                claimed.add(nxt)
+            end = nxt
+            c = consumers[end]
+            nxt = c[0] if len(c) == 1 else None
+        if gate_k is not None:
+            x.append(src(gate_k))
+        if not chain.layers:  # a Dropout with a noise_shape
+            return k, G.Adapter(NO.DropoutOp(nodes[k].layer), x, k)
+        res = add_k = None
+        if nxt is not None and nxt not in claimed and isinstance(nodes[nxt].layer, L.Add):
+            other = [idx[id(i)] for i in nodes[nxt].inputs if idx[id(i)] != end]
+            if len(nodes[nxt].inputs) == 2 and len(other) == 1 and other[0] < k:
+                res, add_k = src(other[0]), nxt
+                claimed.add(nxt)
+                end = nxt
+        if add_k is None and len(chain.layers) == 1 and chain.drop is not None:
+            return k, G.Adapter(NO.DropoutOp(nodes[k].layer), x, k)
+        return at, close(chain, end, x, res, add_k)
+
     for k, t in enumerate(nodes):
+        if k in later:
+            op = later.pop(k)
+            op.inputs = [src(i) for i in op.inputs]
+            ops.append(op)
         if k == input_idx or k in claimed:
             continue
         layer = t.layer
@@ -192,6 +280,17 @@ def _lower(nodes: list, input_idx: int) -> list:
         if isinstance(layer, L.MaxPooling2D):
             ops.append(G.GraphOp(G.MaxPoolOp(layer, pad_of.get(k, 0)), [src(ins[0])], k))
             continue
+        if isinstance(layer, (L.LayerNormalization, L.RMSNormalization, L.LayerScale, L.Multiply, L.Rescaling,
+                              L.Dropout)):
+            at, op = block_boundary(k, ins)
+            if at == k:
+                ops.append(op)
+            else:
+                later[at] = op
+            continue
+        if isinstance(layer, L.Add) and len(ins) == 2 and norm_of(k) is not None:
+            ops.append(close(NO.Chain(), k, [src(ins[1])], src(ins[0]), k))
+            continue
         if isinstance(layer, L.Add):
             relu = False
             end = k
@@ -216,6 +315,7 @@ def _lower(nodes: list, input_idx: int) -> list:
         if inner is None:
             raise NotImplementedError(f"functional lowering of {type(layer).__name__}")
         ops.append(G.Adapter(inner(layer), [src(ins[0])], k))
+    NO.bind_drop_state(ops)
     _bn_bwd_links(ops)
     # dense relu-mask hand-off as in the Sequential engine
     for a, b in zip(ops, ops[1:]):

@@ -82,6 +82,18 @@ class Layer:
     def set_keras_weights(self, ws: list) -> None:
         pass
 
+    def saved_weights(self) -> dict:
+        """{key: array} of a saved model: the Keras weights by their index."""
+        return {str(i): np.ascontiguousarray(w.astype(np.float32)) for i, w in enumerate(self.keras_weights())}
+
+    def load_weights(self, get) -> None:
+        """Take what :meth:`saved_weights` gave; ``get(key)`` returns an array or None."""
+        ws = []
+        while get(str(len(ws))) is not None:
+            ws.append(get(str(len(ws))))
+        if ws:
+            self.set_keras_weights(ws)
+
 
 class Input(Layer):
     kind = "Input"
@@ -108,6 +120,8 @@ class Dense(Layer):
         self.units = int(units)
         self.activation = activation or "linear"
         self.use_bias = use_bias
+        self.quantization = None  # {"mode": "int4", "block_size", "zero_point"} once quantized
+        self.int4 = None  # ops.quant.Int4Weight that inference runs on
 
     def compute_output_shape(self, s):
         return (*s[:-1], self.units)
@@ -126,7 +140,61 @@ class Dense(Layer):
         return self.out_shape
 
     def get_config(self):
-        return {"name": self.name, "units": self.units, "activation": self.activation, "use_bias": self.use_bias}
+        cfg = {"name": self.name, "units": self.units, "activation": self.activation, "use_bias": self.use_bias}
+        return {**cfg, "quantization": dict(self.quantization)} if self.quantization else cfg
+
+    # ---- 4-bit weights (inference): codes and scales replace the kernel, whose fp32 master takes the
+    # values they stand for
+    def can_quantize(self, block_size: int) -> bool:
+        """A layer wide enough for the matrix-core path with whole groups of inputs."""
+        return self.units > 64 and self.units % 8 == 0 and self.fan_in % block_size == 0
+
+    def quantize(self, mode: str = "int4", block_size: int = 128, zero_point: bool = False) -> None:
+        from ..ops import quant as Q
+
+        if mode != "int4":
+            raise NotImplementedError(f"Dense.quantize({mode!r}): int4 only")
+        if self.int4 is not None:
+            raise ValueError(f"{self.name} is quantized already")
+        if not self.can_quantize(block_size):
+            raise ValueError(f"{self.name}: int4 takes more than 64 units, a multiple of 8, and whole groups of "
+                             f"{block_size} inputs (got {self.units} units of {self.fan_in} inputs)")
+        self._set_int4(*Q.int4_quantize(self.kernel.data, block_size, zero_point), block_size)
+
+    def _set_int4(self, codes, scale, zero, group) -> None:
+        from ..ops import quant as Q
+
+        self.int4 = Q.int4_layout(codes, scale, zero, group)
+        self.quantization = {"mode": "int4", "block_size": int(group), "zero_point": zero is not None}
+        w = Q.int4_dequantize(self.int4)
+        self.kernel.data.copy_(w)
+        self.kernel.bf16.copy_(w)
+
+    def saved_weights(self) -> dict:
+        if self.int4 is None:
+            return super().saved_weights()
+        from ..ops import quant as Q
+
+        codes, scale, zero = Q.int4_codes(self.int4)
+        out = {"int4_codes": codes.cpu().numpy(), "int4_scale": scale.float().cpu().numpy()}
+        if zero is not None:
+            out["int4_zero"] = zero.cpu().numpy()
+        if self.bias is not None:
+            out["1"] = self.bias.data.detach().float().cpu().numpy().copy()
+        return out
+
+    def load_weights(self, get) -> None:
+        codes = get("int4_codes")
+        if codes is None:
+            return super().load_weights(get)
+        import torch
+
+        dev = self.kernel.data.device
+        to = lambda a: None if a is None else torch.from_numpy(np.ascontiguousarray(a)).to(dev)  # noqa: E731
+        if self.bias is not None:
+            self.bias.data.copy_(to(get("1")))
+        self._set_int4(to(codes), to(get("int4_scale")).to(torch.bfloat16), to(get("int4_zero")),
+                       int((self.quantization or {}).get("block_size", 128)))
 
     def keras_weights(self):
         out = [self.kernel.data.detach().float().cpu().numpy().T.copy()]
@@ -404,9 +472,176 @@ class ReLU(Layer):
     keras_class = "ReLU"
 
 
+class Dropout(Layer):
+    """Keras ``Dropout``: in training each entry is dropped with probability ``rate`` (to 2**-17) and the
+    rest scaled up; identity in inference.  The mask comes from a counter-based generator over (seed,
+    training step, element) and is never stored.  ``noise_shape`` (batch axis included, None or 1
+    where shared, e.g. ``(None, 1, 1, None)``): one run of axes may share a mask entry.  ``seed`` None
+    derives one from the weight-initialisation seed and the layer's name."""
+
+    kind = "Dropout"
+    keras_class = "Dropout"
+
+    def __init__(self, rate, noise_shape=None, seed=None, name=None):
+        super().__init__(name)
+        if not 0.0 <= float(rate) <= 1.0:
+            raise ValueError(f"Dropout: rate must lie in [0, 1], got {rate}")
+        self.rate = float(rate)
+        self.noise_shape = None if noise_shape is None else tuple(None if v is None else int(v) for v in noise_shape)
+        self.seed = None if seed is None else int(seed)
+
+    def compute_output_shape(self, s):
+        if self.noise_shape is not None:
+            from ..ops.dropout import noise_dims
+
+            lead = self.noise_shape[0] if self.noise_shape else None
+            noise_dims((lead if lead is not None else 2, *s), self.noise_shape)  # refuses what does not fit
+        return tuple(s)
+
+    def seed_value(self) -> int:
+        if self.seed is not None:
+            return self.seed
+        import zlib
+
+        from .. import config
+        from ..ops.dropout import mix_seed
+
+        return mix_seed(config.get("seed"), zlib.crc32(self.name.encode()))
+
+    def get_config(self):
+        return {"name": self.name, "rate": self.rate, "seed": self.seed,
+                "noise_shape": None if self.noise_shape is None else list(self.noise_shape)}
+
+
+class _RowNorm(Layer):
+    """Normalisation of every row of the last axis, with affine parameters [C]."""
+
+    beta = None
+
+    def _eps(self, epsilon):
+        if not float(epsilon) > 0.0:
+            raise ValueError(f"{self.keras_class}: epsilon must be positive, got {epsilon}")
+        return float(epsilon)
+
+    @staticmethod
+    def _axis(axis, who):
+        if axis not in (-1, [-1], (-1,)):
+            raise NotImplementedError(f"{who} over the last axis only")
+
+    def keras_weights(self):
+        return [p.data.detach().float().cpu().numpy().copy() for p in self.params]
+
+    def set_keras_weights(self, ws):
+        import torch
+
+        for p, w in zip(self.params, ws):
+            p.data.copy_(torch.from_numpy(np.ascontiguousarray(w)))
+
+
+class LayerNormalization(_RowNorm):
+    """Keras ``LayerNormalization`` over the last axis (biased variance, epsilon 1e-3)."""
+
+    kind = "LayerNormalization"
+    keras_class = "LayerNormalization"
+    norm_kind = "layer"
+
+    def __init__(self, axis=-1, epsilon=1e-3, center=True, scale=True, name=None):
+        super().__init__(name)
+        self._axis(axis, self.keras_class)
+        self.epsilon, self.center, self.scale = self._eps(epsilon), bool(center), bool(scale)
+
+    def build(self, in_shape, store):
+        super().build(in_shape, store)
+        C = int(in_shape[-1])
+        self.gamma = store.add(f"{self.name}/gamma", (C,), ones) if self.scale else None
+        self.beta = store.add(f"{self.name}/beta", (C,), zeros) if self.center else None
+        self.params = [p for p in (self.gamma, self.beta) if p is not None]
+        return self.out_shape
+
+    def get_config(self):
+        return {"name": self.name, "axis": -1, "epsilon": self.epsilon, "center": self.center, "scale": self.scale}
+
+
+class RMSNormalization(_RowNorm):
+    """Keras ``RMSNormalization`` over the last axis (epsilon 1e-6, a scale and no offset)."""
+
+    kind = "RMSNormalization"
+    keras_class = "RMSNormalization"
+    norm_kind = "rms"
+
+    def __init__(self, axis=-1, epsilon=1e-6, name=None):
+        super().__init__(name)
+        self._axis(axis, self.keras_class)
+        self.epsilon = self._eps(epsilon)
+
+    def build(self, in_shape, store):
+        super().build(in_shape, store)
+        self.gamma = store.add(f"{self.name}/scale", (int(in_shape[-1]),), ones)
+        self.params = [self.gamma]
+        return self.out_shape
+
+    def get_config(self):
+        return {"name": self.name, "axis": -1, "epsilon": self.epsilon}
+
+
+class LayerScale(_RowNorm):
+    """A trained gate per channel on a residual branch: y = x * gamma, gamma starting at
+    ``init_values``."""
+
+    kind = "LayerScale"
+    keras_class = "LayerScale"
+
+    def __init__(self, init_values=1e-5, name=None):
+        super().__init__(name)
+        self.init_values = float(init_values)
+
+    def build(self, in_shape, store):
+        super().build(in_shape, store)
+        self.gamma = store.add(f"{self.name}/gamma", (int(in_shape[-1]),),
+                               lambda shape, rng: np.full(shape, self.init_values, np.float32))
+        self.params = [self.gamma]
+        return self.out_shape
+
+    def get_config(self):
+        return {"name": self.name, "init_values": self.init_values}
+
+
+class Rescaling(Layer):
+    """Keras ``Rescaling`` without an offset: y = x * scale (the residual scale of a block)."""
+
+    kind = "Rescaling"
+    keras_class = "Rescaling"
+
+    def __init__(self, scale, offset=0.0, name=None):
+        super().__init__(name)
+        if float(offset) != 0.0:
+            raise NotImplementedError("Rescaling with an offset")
+        self.scale = float(scale)
+
+    def get_config(self):
+        return {"name": self.name, "scale": self.scale, "offset": 0.0}
+
+
+class Multiply(Layer):
+    """Keras ``Multiply`` of [branch, gate]: a gate of the branch's shape, or one row of channels per
+    sample for a branch of several rows a sample."""
+
+    kind = "Multiply"
+    keras_class = "Multiply"
+
+    def compute_output_shape(self, s):
+        if not s or not isinstance(s[0], tuple) or len(s) != 2:
+            raise NotImplementedError("Multiply of exactly two tensors")
+        a, g = s
+        if tuple(g) != tuple(a) and tuple(g) != (a[-1],):
+            raise ValueError(f"Multiply: a gate of shape {g} does not fit a branch of shape {a}")
+        return tuple(a)
+
+
 LAYER_CLASSES = {c.keras_class: c for c in (Input, Dense, Conv2D, PReLU, MaxPooling2D, Flatten,
                                               GlobalAveragePooling2D, ReLU, ZeroPadding2D, BatchNormalization,
-                                              Activation, Add)}
+                                              Activation, Add, Dropout, LayerNormalization,
+                                              RMSNormalization, LayerScale, Rescaling, Multiply)}
 
 
 def layer_from_config(cls_name: str, cfg: dict) -> Layer:
@@ -415,7 +650,9 @@ def layer_from_config(cls_name: str, cfg: dict) -> Layer:
     if cls is Input:
         return Input(cfg["batch_shape"][1:], name=cfg.get("name"))
     if cls is Dense:
-        return Dense(cfg["units"], cfg.get("activation"), cfg.get("use_bias", True), name=cfg.get("name"))
+        d = Dense(cfg["units"], cfg.get("activation"), cfg.get("use_bias", True), name=cfg.get("name"))
+        d.quantization = cfg.get("quantization")
+        return d
     if cls is Conv2D:
         return Conv2D(cfg["filters"], tuple(cfg["kernel_size"]), tuple(cfg.get("strides", (1, 1))),
                       cfg.get("padding", "valid"), cfg.get("activation"), cfg.get("use_bias", True),
@@ -431,10 +668,21 @@ def layer_from_config(cls_name: str, cfg: dict) -> Layer:
                                   center=cfg.get("center", True), scale=cfg.get("scale", True), name=cfg.get("name"))
     if cls is Activation:
         return Activation(cfg["activation"], name=cfg.get("name"))
+    if cls is Dropout:
+        return Dropout(cfg["rate"], cfg.get("noise_shape"), cfg.get("seed"), name=cfg.get("name"))
+    if cls is LayerNormalization:
+        return LayerNormalization(epsilon=cfg.get("epsilon", 1e-3), center=cfg.get("center", True),
+                                  scale=cfg.get("scale", True), name=cfg.get("name"))
+    if cls is RMSNormalization:
+        return RMSNormalization(epsilon=cfg.get("epsilon", 1e-6), name=cfg.get("name"))
+    if cls is LayerScale:
+        return LayerScale(cfg.get("init_values", 1e-5), name=cfg.get("name"))
+    if cls is Rescaling:
+        return Rescaling(cfg["scale"], cfg.get("offset", 0.0), name=cfg.get("name"))
     return cls(name=cfg.get("name"))
 
 
 __all__ = ["Layer", "Input", "Dense", "Conv2D", "PReLU", "MaxPooling2D", "Flatten", "GlobalAveragePooling2D",
-           "ReLU", "ZeroPadding2D", "BatchNormalization", "Activation", "Add", "layer_from_config",
-           "reset_name_counters"]
+           "ReLU", "ZeroPadding2D", "BatchNormalization", "Activation", "Add", "Dropout", "LayerNormalization",
+           "RMSNormalization", "LayerScale", "Rescaling", "Multiply", "layer_from_config", "reset_name_counters"]
 

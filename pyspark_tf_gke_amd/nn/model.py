@@ -77,6 +77,8 @@ class Variable:
         return self.param.data.detach().cpu().numpy()
 
     def assign(self, value):
+        if getattr(self.model, "quantized", False):
+            raise RuntimeError("a quantized model's weights cannot be assigned")
         self.param.data.copy_(torch.as_tensor(value, dtype=torch.float32))
 
 
@@ -97,6 +99,7 @@ class Sequential:
         self._eval_stats = None
         self.stop_training = False
         self.strategy = None
+        self._quantized = False
         for l in layers or []:
             self.add(l)
 
@@ -154,7 +157,48 @@ class Sequential:
         self._check_master()
         return [w for l in self.layers for w in l.keras_weights()]
 
+    @property
+    def quantized(self) -> bool:
+        """Some layer runs on 4-bit weights: the model is for inference."""
+        return self._quantized
+
+    def quantize(self, mode: str = "int4", block_size: int = 128, zero_point: bool = False) -> None:
+        """Keras ``model.quantize("int4")``: every Dense layer of more than 64 units (a multiple of 8) whose
+        inputs divide into groups of ``block_size`` (32, 64 or 128) keeps 4-bit weights with a bf16 scale,
+        and with ``zero_point`` a zero point, for each group; the others stay as they are.  The
+        model then is for inference: ``predict`` / ``evaluate`` read a quarter of the bf16 weight bytes,
+        and training, ``set_weights`` and checkpoints are refused.  ``save`` keeps the codes."""
+        from ..ops import quant as Q
+
+        if mode != "int4":
+            raise NotImplementedError(f"quantize({mode!r}): int4 only")
+        if block_size not in Q.GROUPS:
+            raise ValueError(f"quantize: block_size must be one of {Q.GROUPS}, got {block_size}")
+        if not self.built:
+            raise ValueError("quantize: build the model first")
+        if self.quantized:
+            raise ValueError("quantize: the model is quantized already")
+        self._check_master()
+        if getattr(self, "_lazy_dw", None):
+            from .tape import flush_lazy
+
+            flush_lazy(self)
+        todo = [l for l in self.layers if isinstance(l, L.Dense) and l.can_quantize(block_size)]
+        if not todo:
+            raise ValueError(f"quantize: no Dense layer of more than 64 units (a multiple of 8) takes whole groups of "
+                             f"{block_size} inputs")
+        for l in todo:
+            l.quantize(mode, block_size, zero_point)
+        self._quantized = True
+        self.store.flip_token = None
+        self._graphs, self._graph_warm = {}, {}  # captured training steps
+
+    def _refuse_quantized(self, what: str) -> None:
+        if self._quantized:
+            raise RuntimeError(f"{what}: the model is quantized (inference only)")
+
     def set_weights(self, ws):
+        self._refuse_quantized("set_weights")
         i = 0
         for l in self.layers:
             n = len(l.keras_weights())
@@ -287,6 +331,8 @@ class Sequential:
         from .tape import _active_tape
 
         tape = _active_tape()
+        if training or tape is not None:
+            self._refuse_quantized("training forward")
         if tape is not None and training and self._tape_head_ok():
             out = self._tape_head_forward(xb)
             tape.record_forward(self, out)
@@ -570,6 +616,7 @@ class Sequential:
         store.grad_clean = True
 
     def train_step(self, xb, yb, stats=None) -> None:
+        self._refuse_quantized("train_step")
         _fault.maybe_fail()
         _heartbeat.progress()
         st = self._strategy()
@@ -595,6 +642,7 @@ class Sequential:
     def train_step_fast(self, xb, yb, stats=None) -> None:
         """One training step; replays a captured HIP graph when ``jit_compile`` is on (same batch
         shape/dtype as the captured step), otherwise runs eagerly."""
+        self._refuse_quantized("train_step")
         stats = self._stats_buf() if stats is None else stats
         if not self._graph_usable(xb):
             return self.train_step(xb, yb, stats)
@@ -866,8 +914,8 @@ class Sequential:
                 "date_saved": time.strftime("%Y-%m-%d@%H:%M:%S"), "weights_format": "safetensors"}
         tensors = {}
         for l in self.layers:
-            for i, w in enumerate(l.keras_weights()):
-                tensors[f"layers/{l.name}/vars/{i}"] = np.ascontiguousarray(w.astype(np.float32))
+            for k, w in l.saved_weights().items():
+                tensors[f"layers/{l.name}/vars/{k}"] = w
         os.makedirs(os.path.dirname(os.path.abspath(filepath)) or ".", exist_ok=True)
         tmp = filepath + ".tmp"
         with zipfile.ZipFile(tmp, "w") as zf:
@@ -894,13 +942,8 @@ def load_model(filepath: str, compile: bool = True, device=None) -> Sequential:
             m.add(L.layer_from_config(lc["class_name"], lc["config"]))
     m.build(device=device)
     for l in m.layers:
-        ws = []
-        i = 0
-        while f"layers/{l.name}/vars/{i}" in tensors:
-            ws.append(tensors[f"layers/{l.name}/vars/{i}"])
-            i += 1
-        if ws:
-            l.set_keras_weights(ws)
+        l.load_weights(lambda k, n=l.name: tensors.get(f"layers/{n}/vars/{k}"))
+    m._quantized = any(getattr(l, "int4", None) is not None for l in m.layers)
     m.store.refresh_bf16()
     cc = cfg.get("compile_config") or {}
     if compile and cc.get("loss"):

@@ -67,10 +67,10 @@ def save(model, export_dir: str, signatures=None, assets: dict | None = None) ->
     os.makedirs(os.path.join(tmp, "assets"))
     tensors, index = {}, {}
     for l in model.layers:
-        for i, w in enumerate(l.keras_weights()):
-            key = f"{l.name}/{i}"
-            tensors[key] = np.ascontiguousarray(np.asarray(w, dtype=np.float32))
-            index[key] = {"shape": list(tensors[key].shape), "dtype": "float32"}
+        for k, w in l.saved_weights().items():
+            key = f"{l.name}/{k}"
+            tensors[key] = w
+            index[key] = {"shape": list(w.shape), "dtype": str(w.dtype)}
     save_file(tensors, os.path.join(tmp, "variables", "variables.safetensors"))
     with open(os.path.join(tmp, "variables", "variables.index.json"), "w") as fh:
         json.dump(index, fh, indent=1)
@@ -139,11 +139,7 @@ def load(export_dir: str, device=None) -> LoadedModel:
     m.build(device=device)
     tensors = load_file(os.path.join(export_dir, "variables", "variables.safetensors"))
     for l in m.layers:
-        ws, i = [], 0
-        while f"{l.name}/{i}" in tensors:
-            ws.append(tensors[f"{l.name}/{i}"])
-            i += 1
-        if ws:
-            l.set_keras_weights(ws)
+        l.load_weights(lambda k, n=l.name: tensors.get(f"{n}/{k}"))
+    m._quantized = any(getattr(l, "int4", None) is not None for l in m.layers)
     m.store.refresh_bf16()
     return LoadedModel(m, meta)

@@ -1,6 +1,6 @@
 """Checkpoint / resume.  The reference only saves the final ``model.keras``; here a
 checkpoint holds the fp32 parameters (per parameter name), the optimizer state (Adam moments / SGD velocity) and
-step, the BatchNormalization moving statistics, the epoch, and every rank's RNG state, written
+step, the BatchNormalization moving statistics, the step of the dropout masks, the epoch, and every rank's RNG state, written
 atomically with safetensors + a JSON manifest.  Parameters/moments are stored once, per parameter
 name, in the full layout (rank 0 writes them after the strategy gathered any sharded state); each
 rank writes its own RNG file.
@@ -30,6 +30,8 @@ def save_checkpoint(model, path: str, epoch: int, extra: dict | None = None) -> 
     distinct random streams across a resume."""
     from safetensors.torch import save_file
 
+    if getattr(model, "quantized", False):
+        raise RuntimeError("checkpoints hold training state: the model is quantized (use save())")
     os.makedirs(path, exist_ok=True)
     opt = model.optimizer
     st = model.store
@@ -62,7 +64,7 @@ def save_checkpoint(model, path: str, epoch: int, extra: dict | None = None) -> 
     comm.barrier()
     if rank == 0:
         manifest = {"epoch": epoch, "step": opt.iterations if opt else 0, "world_size": comm.world_size(),
-                    "sharded": False, "layout": "per-param", "total": int(st.total), "time": time.time(),
+                    "drop_step": _drop_step(model), "sharded": False, "layout": "per-param", "total": int(st.total), "time": time.time(),
                     **(extra or {})}
         with open(os.path.join(path, "manifest.json.tmp"), "w") as fh:
             json.dump(manifest, fh)
@@ -71,8 +73,18 @@ def save_checkpoint(model, path: str, epoch: int, extra: dict | None = None) -> 
     return path
 
 
+def _drop_step(model) -> int:
+    from ..nn.norm_ops import drop_state
+
+    st = drop_state(model.ops)
+    return 0 if st is None else st.get()
+
+
 def load_checkpoint(model, path: str) -> dict:
     from safetensors import safe_open
+
+    if getattr(model, "quantized", False):
+        raise RuntimeError("checkpoints hold training state: the model is quantized")
 
     with open(os.path.join(path, "manifest.json")) as fh:
         manifest = json.load(fh)
@@ -115,6 +127,11 @@ def load_checkpoint(model, path: str) -> dict:
         torch.cuda.set_rng_state(rng["rng/cuda"], st.flat.device)
     if opt is not None:
         opt.set_iterations(int(manifest["step"]))
+    from ..nn.norm_ops import drop_state
+
+    ds = drop_state(model.ops)
+    if ds is not None:  # the next training pass draws the masks an uninterrupted run would draw
+        ds.set(int(manifest.get("drop_step", 0)))
     st.refresh_bf16()
     st.master_stale = False
     if strat is not None and hasattr(strat, "on_state_loaded"):

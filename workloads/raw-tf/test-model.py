@@ -21,8 +21,10 @@ IMG_W, IMG_H = 320, 256
 
 
 class ManualImageChecker:
-    def __init__(self, model_path, plots_dir, device=None):
+    def __init__(self, model_path, plots_dir, device=None, quantize=None):
         self.model = load_model(model_path, device=device)
+        if quantize and not self.model.quantized:
+            self.model.quantize(quantize)
         self.model.summary()
         self.plots_dir = plots_dir
         os.makedirs(plots_dir, exist_ok=True)
@@ -63,9 +65,11 @@ def main(argv=None):
     ap.add_argument("--images", default="./images")
     ap.add_argument("--sleep", type=float, default=0.0)
     ap.add_argument("--device", default=None)
+    ap.add_argument("--quantize", default=None, choices=["int4"],
+                    help="answer from 4-bit Dense weights (one image reads a quarter of the weight bytes)")
     a = ap.parse_args(argv)
     model = a.model or os.path.join(a.model_dir, "150-320-by-256-B1-model.keras")
-    ManualImageChecker(model, os.path.join(a.model_dir, "plots"), a.device).run(a.images, a.sleep)
+    ManualImageChecker(model, os.path.join(a.model_dir, "plots"), a.device, a.quantize).run(a.images, a.sleep)
 
 
 if __name__ == "__main__":
