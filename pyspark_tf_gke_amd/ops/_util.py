@@ -38,8 +38,9 @@ def hip(name: str, *args) -> None:
 
 def hip_on(device: torch.device, name: str, *args) -> None:
     """:func:`hip` on the current stream of ``device``, which need not be the current device."""
-    if _CUR_DEVICE is not None and device.index == _CUR_DEVICE():
-        _native.call(name, *args, stream_handle())
+    index = device.index
+    if _RAW_STREAM is not None and _CUR_DEVICE is not None and index == _CUR_DEVICE():
+        _native.call(name, *args, _RAW_STREAM(index))
         return
     with torch.cuda.device(device):
         _native.call(name, *args, stream_handle())

@@ -35,7 +35,6 @@ class Drop(NamedTuple):
 
 def threshold(rate: float) -> tuple[int, float]:
     """(threshold of the 16-bit pieces, scale of what is kept)."""
-    rate = float(rate)
     if not 0.0 <= rate <= 1.0:  # also refuses NaN
         raise ValueError(f"dropout: rate must lie in [0, 1], got {rate}")
     thr = int(round(rate * 65536))
@@ -114,28 +113,24 @@ def keep_mask(shape, rate: float, seed: int, step, noise_shape=None) -> torch.Te
 
 def _run(name, x, rate, seed, step, out, noise_shape):
     thr, scale = threshold(rate)
-    if x.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"{name}: expected bfloat16 or float32, got {x.dtype}")
-    if out.dtype != x.dtype or out.shape != x.shape or out.device != x.device:
+    dt = x.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float32:
+        raise TypeError(f"{name}: expected bfloat16 or float32, got {dt}")
+    if out.dtype is not dt or out.shape != x.shape or out.device != x.device:
         raise ValueError(f"{name}: output must match the input's shape, dtype and device")
     if not x.is_contiguous() or not out.is_contiguous():
         raise ValueError(f"{name}: tensor must be contiguous")
-    _, mid, inner = noise_dims(x.shape, noise_shape)
+    mid, inner = (1, 1) if noise_shape is None else noise_dims(x.shape, noise_shape)[1:]
     host, dev = step_args(step, x.device)
-    if not on_device(x):
+    if not x.is_cuda:
         keep = keep_mask(x.shape, rate, seed, step, noise_shape)
-        out.copy_(torch.where(keep, x.float() * scale, 0.0).to(out.dtype))
+        out.copy_(torch.where(keep, x.float() * scale, 0.0).to(dt))
         return out
-    if out.data_ptr() != x.data_ptr() and _overlap(x, out):
+    xp, op, n, f32 = x.data_ptr(), out.data_ptr(), x.numel(), dt is torch.float32
+    if xp != op and abs(xp - op) < n * (4 if f32 else 2):
         raise ValueError(f"{name}: input and output overlap")
-    hip_on(x.device, "ptg_dropout", ptr(x), ptr(out), x.numel(), int(x.dtype == torch.float32), thr, scale,
-           _signed(seed), host, ptr(dev), mid, inner)
+    hip_on(x.device, "ptg_dropout", xp, op, n, f32, thr, scale, _signed(seed), host, ptr(dev), mid, inner)
     return out
-
-
-def _overlap(a, b) -> bool:
-    size = a.numel() * a.element_size()
-    return a.data_ptr() < b.data_ptr() + size and b.data_ptr() < a.data_ptr() + size
 
 
 def dropout_fwd(x, rate: float, seed: int, step, out, noise_shape=None):

@@ -24,7 +24,7 @@ from typing import NamedTuple
 import torch
 
 from . import dropout as DR
-from ._util import hip_on, on_device, ptr
+from ._util import hip_on, ptr
 
 KINDS = {"layer": 1, "rms": 2}
 MAX_COLS = 8192
@@ -50,115 +50,146 @@ def block_norm_workspace(rows: int, cols: int, groups: int, device) -> torch.Ten
     two streams, or in two captured graphs - need one each."""
     if torch.device(device).type != "cuda" or rows == 0:
         return torch.empty(0, dtype=torch.float32, device=device)
-    from .. import _native
-
     if not 1 <= cols <= MAX_COLS:
         raise ValueError(f"block_norm: rows of 1..{MAX_COLS} columns, got {cols}")
     if groups < 1 or rows % groups:
         raise ValueError(f"block_norm: {rows} rows do not divide into {groups} gate groups")
-    n = ctypes.c_long(0)
-    _native.check(_native.hip_lib().ptg_block_norm_ws(rows, cols, groups, ctypes.byref(n)), "ptg_block_norm_ws")
-    return torch.empty(n.value, dtype=torch.float32, device=device)
+    return torch.empty(block_norm_workspace_floats(rows, cols, groups), dtype=torch.float32, device=device)
 
 
-def _same(t, like, name):
-    if t is None:
-        return
-    if t.dtype != like.dtype or t.shape != like.shape or t.device != like.device:
-        raise ValueError(f"block_norm: {name} must match x in shape, dtype and device")
-    if not t.is_contiguous():
-        raise ValueError(f"block_norm: {name} must be contiguous")
+_NO_DROP = (0, 0, 1.0, 0, 0, None)  # on, threshold, scale, seed, host step, device step
+
+
+def _bad(name, x):
+    raise ValueError(f"block_norm: {name} must be contiguous and match x ({tuple(x.shape)}, {x.dtype}, {x.device})")
 
 
 def _vec(t, C, dev, name):
-    if t is None:
-        return
-    if t.dtype != torch.float32:
+    if t.dtype is not torch.float32:
         raise TypeError(f"block_norm: {name} must be float32, got {t.dtype}")
-    if tuple(t.shape) != (C,) or t.device != dev or not t.is_contiguous():
+    if t.dim() != 1 or t.shape[0] != C or t.device != dev or not t.is_contiguous():
         raise ValueError(f"block_norm: {name} must be a contiguous [{C}] vector on {dev}")
 
 
-def _check_norm(nm, C, dev, name):
+def _norm_args(nm, C, dev, name):
+    """(kind, gamma pointer, beta pointer, epsilon), checked."""
     if nm is None:
-        return
-    if nm.kind not in KINDS:
+        return 0, None, None, 0.0
+    kind = KINDS.get(nm.kind)
+    if kind is None:
         raise ValueError(f"block_norm: {name} kind {nm.kind!r} (layer or rms)")
-    if not float(nm.eps) > 0.0:
+    g, b, eps = nm.gamma, nm.beta, float(nm.eps)
+    if not eps > 0.0:
         raise ValueError(f"block_norm: {name} needs an epsilon > 0, got {nm.eps}")
-    if nm.kind == "rms" and nm.beta is not None:
-        raise ValueError(f"block_norm: {name}: an RMSNorm has no beta")
-    _vec(nm.gamma, C, dev, name + ".gamma")
-    _vec(nm.beta, C, dev, name + ".beta")
+    if g is not None:
+        _vec(g, C, dev, name + ".gamma")
+        g = g.data_ptr()
+    if b is not None:
+        if kind == 2:
+            raise ValueError(f"block_norm: {name}: an RMSNorm has no beta")
+        _vec(b, C, dev, name + ".beta")
+        b = b.data_ptr()
+    return kind, g, b, eps
 
 
-def _gate_dims(gate, x, M, C):
-    """(mode, rows per gate row)."""
-    if gate is None:
-        return 0, 1
-    if gate.dim() == 1:
-        _vec(gate, C, x.device, "gate")
-        return 1, max(M, 1)
-    if gate.dim() != 2 or gate.shape[1] != C or gate.dtype != x.dtype or gate.device != x.device \
-            or not gate.is_contiguous():
-        raise ValueError(f"block_norm: gate must be fp32 [{C}] or {x.dtype} [groups, {C}], contiguous, on {x.device}")
-    G = gate.shape[0]
-    if M and (G == 0 or M % G):
-        raise ValueError(f"block_norm: {M} rows do not divide into {G} gate groups")
-    return 2, M // G if G else 1
-
-
-def _common(x, res, post, gate, drop, pre):
-    if x.dtype not in (torch.bfloat16, torch.float32):
+def _common(x, gate, drop):
+    """(rows, columns, gate mode, rows per gate row, dropout arguments), checked."""
+    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float32:
         raise TypeError(f"block_norm: expected bfloat16 or float32, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("block_norm: x needs at least one column")
     if not x.is_contiguous():
         raise ValueError("block_norm: x must be contiguous")
-    C = x.shape[-1]
+    C, dev = x.shape[-1], x.device
     M = x.numel() // C
     if C > MAX_COLS and x.is_cuda:
         raise ValueError(f"block_norm: rows of at most {MAX_COLS} columns, got {C}")
-    _same(res, x, "res")
-    _check_norm(post, C, x.device, "post")
-    _check_norm(pre, C, x.device, "pre")
-    mode, rpg = _gate_dims(gate, x, M, C)
-    d = (0, 0, 1.0, 0, 0, None)  # on, threshold, scale, seed, host step, device step
-    if drop is not None:
-        thr, ds = DR.threshold(drop.rate)
-        host, dev = DR.step_args(drop.step, x.device)
-        d = (1, thr, ds, DR._signed(drop.seed), host, dev)
-    return M, C, mode, rpg, d
+    mode, rpg = 0, 1
+    if gate is not None:
+        if gate.dim() == 1:
+            _vec(gate, C, dev, "gate")
+            mode, rpg = 1, M or 1
+        else:
+            if gate.dim() != 2 or gate.shape[1] != C or gate.dtype is not x.dtype or gate.device != dev \
+                    or not gate.is_contiguous():
+                raise ValueError(f"block_norm: gate must be fp32 [{C}] or {x.dtype} [groups, {C}], contiguous, on {dev}")
+            G = gate.shape[0]
+            if M and (G == 0 or M % G):
+                raise ValueError(f"block_norm: {M} rows do not divide into {G} gate groups")
+            mode, rpg = 2, M // G if G else 1
+    if drop is None:
+        return M, C, mode, rpg, _NO_DROP
+    thr, ds = DR.threshold(drop.rate)
+    host, step = DR.step_args(drop.step, dev)
+    return M, C, mode, rpg, (1, thr, ds, DR._signed(drop.seed), host, step)
+
+
+def _pointers(x, tensors, names):
+    """Data pointers of the tensors that must look like x (None where absent)."""
+    out, dt, shp, dev = [], x.dtype, x.shape, x.device
+    for t, name in zip(tensors, names):
+        if t is None:
+            out.append(None)
+            continue
+        if t.dtype is not dt or t.shape != shp or t.device != dev or not t.is_contiguous():
+            _bad(name, x)
+        out.append(t.data_ptr())
+    return out
+
+
+def _apart(outs, ins, size):
+    """No output may overlap an input (pointer, name, whether the very same buffer will do) or another
+    output.  Every element is read before it is written, by the same thread."""
+    for k, (o, on) in enumerate(outs):
+        for i, iname, same in ins:
+            if -size < o - i < size and not (o == i and same):
+                raise ValueError(f"block_norm: {on} overlaps {iname}")
+        for p, pn in outs[:k]:
+            if -size < o - p < size:
+                raise ValueError(f"block_norm: {on} overlaps {pn}")
+
+
+def _gate_apart(gate, outs, size):
+    lo, hi = gate.data_ptr(), gate.data_ptr() + gate.numel() * gate.element_size()
+    for o, on in outs:
+        if lo < o + size and o < hi:
+            raise ValueError(f"block_norm: {on} overlaps gate")
 
 
 def _stats_ok(stats, M, dev):
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (4, M) or stats.device != dev or not stats.is_contiguous():
+    if stats.dtype is not torch.float32 or tuple(stats.shape) != (4, M) or stats.device != dev \
+            or not stats.is_contiguous():
         raise ValueError(f"block_norm: stats must be a contiguous fp32 [4, {M}] on {dev}")
-
-
-def _aligned(C, *ts) -> int:
-    return int(C % 8 == 0 and all(t is None or t.data_ptr() % 16 == 0 for t in ts))
-
-
-def _nk(nm):
-    return 0 if nm is None else KINDS[nm.kind]
 
 
 def block_norm_fwd(x, *, res=None, post=None, gate=None, scale: float = 1.0, drop=None, pre=None, h=None, u=None,
                    stats=None):
     """Writes ``h`` (if given) and ``u`` (with ``pre``); ``stats`` (:func:`block_norm_stats`) for a
-    backward pass.  Returns (h, u).  ``h`` may be ``res``, nothing else may overlap an input."""
-    M, C, mode, rpg, d = _common(x, res, post, gate, drop, pre)
-    _same(h, x, "h")
-    _same(u, x, "u")
+    backward pass.  Returns (h, u).  ``h`` may be ``res`` or ``x``; nothing else may overlap an input."""
+    M, C, mode, rpg, d = _common(x, gate, drop)
+    dev = x.device
     if (pre is None) != (u is None):
         raise ValueError("block_norm: u goes with pre")
     if h is None and u is None:
         raise ValueError("block_norm: nothing to write (h and u are None)")
+    k1, g1, b1, e1 = _norm_args(post, C, dev, "post")
+    k2, g2, b2, e2 = _norm_args(pre, C, dev, "pre")
+    xp = x.data_ptr()
+    rp, hp, up = _pointers(x, (res, h, u), ("res", "h", "u"))
     if stats is not None:
-        _stats_ok(stats, M, x.device)
-    _no_overlap({"x": x, "res": res, "gate": gate}, {"h": h, "u": u}, allow=(("res", "h"), ("x", "h")))
-    if not on_device(x):
+        _stats_ok(stats, M, dev)
+    f32 = x.dtype is torch.float32
+    size = M * C * (4 if f32 else 2)
+    ins = [(xp, "x", True)] if rp is None else [(xp, "x", True), (rp, "res", True)]
+    if up is not None:  # u is written after others have read, and h written before it
+        _apart([(up, "u")], [(i, n, False) for i, n, _ in ins], size)
+    outs = [] if hp is None else [(hp, "h")]
+    if up is not None and hp is not None:
+        outs.append((up, "u"))
+    _apart(outs, ins, size)
+    if mode == 2:
+        _gate_apart(gate, [(p, n) for p, n in ((hp, "h"), (up, "u")) if p is not None], size)
+    if not x.is_cuda:
         hv, uv, st = _ref_fwd(x, res, post, gate, scale, drop, pre, M, C, rpg)
         if h is not None:
             h.copy_(hv.view(x.shape).to(h.dtype))
@@ -167,11 +198,10 @@ def block_norm_fwd(x, *, res=None, post=None, gate=None, scale: float = 1.0, dro
         if stats is not None:
             stats.copy_(st)
         return h, u
-    p, q = post or (None,) * 4, pre or (None,) * 4
-    hip_on(x.device, "ptg_block_norm_fwd", ptr(x), ptr(res), ptr(gate), ptr(h), ptr(u), ptr(p[1]), ptr(p[2]), ptr(q[1]),
-           ptr(q[2]), ptr(stats), M, C, int(x.dtype == torch.float32),
-           _aligned(C, x, res, gate if mode == 2 else None, h, u), _nk(post), float(p[3] or 0.0), _nk(pre),
-           float(q[3] or 0.0), mode, rpg, float(scale), *d[:5], ptr(d[5]))
+    gp = None if gate is None else gate.data_ptr()
+    aligned = C % 8 == 0 and not (xp | (rp or 0) | (hp or 0) | (up or 0) | ((gp or 0) if mode == 2 else 0)) & 15
+    hip_on(dev, "ptg_block_norm_fwd", xp, rp, gp, hp, up, g1, b1, g2, b2, None if stats is None else stats.data_ptr(),
+           M, C, f32, aligned, k1, e1, k2, e2, mode, rpg, scale, d[0], d[1], d[2], d[3], d[4], ptr(d[5]))
     return h, u
 
 
@@ -179,58 +209,70 @@ def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1
                    dh=None, dx=None, dres=None, dgate=None, dpost=None, dpre=None, workspace=None):
     """Gradients of :func:`block_norm_fwd` (same x, res, post, gate, scale, drop, pre) from ``du`` (with
     ``pre``) and ``dh`` (None: zero).  Writes dx and dres (None: skipped), ``dgate`` like ``gate``, and
-    ``dpost`` / ``dpre`` = (dgamma, dbeta), fp32 [C] or None where the norm has none.  ``dres`` may be
-    ``dh``.  ``workspace``: :func:`block_norm_workspace` (None: allocated here)."""
-    M, C, mode, rpg, d = _common(x, res, post, gate, drop, pre)
-    for t, name in ((du, "du"), (dh, "dh"), (dx, "dx"), (dres, "dres")):
-        _same(t, x, name)
+    ``dpost`` / ``dpre`` = (dgamma, dbeta), fp32 [C] or None where the norm has none.  ``dx`` and ``dres``
+    may each be one of x, res, du and dh; nothing else may overlap.  ``workspace``:
+    :func:`block_norm_workspace` (None: allocated here)."""
+    M, C, mode, rpg, d = _common(x, gate, drop)
+    dev = x.device
     if (pre is None) != (du is None):
         raise ValueError("block_norm: du goes with pre")
     if pre is None and dh is None:
         raise ValueError("block_norm: no gradient comes in (du and dh are None)")
     if dx is None and dres is None and dgate is None and dpost is None and dpre is None:
         raise ValueError("block_norm: no gradient is asked for")
-    _stats_ok(stats, M, x.device)
-    if dgate is not None:
-        if gate is None or dgate.shape != gate.shape or dgate.dtype != gate.dtype or dgate.device != x.device \
-                or not dgate.is_contiguous():
-            raise ValueError("block_norm: dgate must match gate")
+    k1, g1, b1, _ = _norm_args(post, C, dev, "post")
+    k2, g2, _, _ = _norm_args(pre, C, dev, "pre")
+    xp = x.data_ptr()
+    rp, up, hp, dxp, drp = _pointers(x, (res, du, dh, dx, dres), ("res", "du", "dh", "dx", "dres"))
+    _stats_ok(stats, M, dev)
+    if dgate is not None and (gate is None or dgate.shape != gate.shape or dgate.dtype is not gate.dtype
+                              or dgate.device != dev or not dgate.is_contiguous()):
+        raise ValueError("block_norm: dgate must match gate")
     vecs = []
     for g, nm, name in ((dpost, post, "dpost"), (dpre, pre, "dpre")):
-        g = g or (None, None)
-        for t, w, part in ((g[0], nm.gamma if nm else None, "gamma"), (g[1], nm.beta if nm else None, "beta")):
-            if t is not None and w is None:
-                raise ValueError(f"block_norm: {name} asks for the gradient of an absent {part}")
-            _vec(t, C, x.device, f"{name}.{part}")
+        if g is None:
+            vecs += (None, None)
+            continue
+        for t, w, part in ((g[0], nm and nm.gamma, "gamma"), (g[1], nm and nm.beta, "beta")):
+            if t is not None:
+                if w is None:
+                    raise ValueError(f"block_norm: {name} asks for the gradient of an absent {part}")
+                _vec(t, C, dev, name)
             vecs.append(t)
-    _no_overlap({"x": x, "res": res, "gate": gate, "du": du, "dh": dh}, {"dx": dx, "dres": dres, "dgate": dgate},
-                allow=(("dh", "dres"), ("du", "dres"), ("du", "dx"), ("dh", "dx"), ("x", "dx"), ("res", "dres"),
-                       ("x", "dres"), ("res", "dx")))
+    f32 = x.dtype is torch.float32
+    size = M * C * (4 if f32 else 2)
+    outs = [(p, n) for p, n in ((dxp, "dx"), (drp, "dres")) if p is not None]
+    _apart(outs, [(p, n, True) for p, n in ((xp, "x"), (rp, "res"), (up, "du"), (hp, "dh")) if p is not None], size)
+    if mode == 2:
+        _gate_apart(gate, outs, size)
+        if dgate is not None:
+            _gate_apart(dgate, outs + [(p, n) for p, n in ((xp, "x"), (rp, "res"), (up, "du"), (hp, "dh"))
+                                       if p is not None], size)
+            _gate_apart(dgate, [(gate.data_ptr(), "gate")], gate.numel() * gate.element_size())
     if M == 0:
         for t in (dgate, *vecs):
             if t is not None:
                 t.zero_()
         return dx, dres
-    if not on_device(x):
+    if not x.is_cuda:
         _ref_bwd(x, stats, res, post, gate, scale, drop, pre, du, dh, dx, dres, dgate, vecs, M, C, rpg)
         return dx, dres
-    groups = M // rpg if mode == 2 else 1
-    need = block_norm_workspace_floats(M, C, groups)
+    need = block_norm_workspace_floats(M, C, M // rpg if mode == 2 else 1)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.float32, device=x.device)
-    elif workspace.dtype != torch.float32 or workspace.device != x.device or workspace.numel() < need \
+        workspace = torch.empty(need, dtype=torch.float32, device=dev)
+    elif workspace.dtype is not torch.float32 or workspace.device != dev or workspace.numel() < need \
             or not workspace.is_contiguous():
-        raise ValueError(f"block_norm: workspace must hold {need} contiguous floats on {x.device}")
-    p, q = post or (None,) * 4, pre or (None,) * 4
+        raise ValueError(f"block_norm: workspace must hold {need} contiguous floats on {dev}")
     if mode == 2 and dgate is None:
-        mode_b, keep = 2, torch.empty_like(gate)  # the kernel writes it; dropped
-    else:
-        mode_b, keep = mode, dgate
-    hip_on(x.device, "ptg_block_norm_bwd", ptr(x), ptr(res), ptr(gate), ptr(du), ptr(dh), ptr(dx), ptr(dres), ptr(p[1]),
-           ptr(p[2]), ptr(q[1]), ptr(stats), *[ptr(t) for t in vecs], ptr(keep), ptr(workspace), M, C,
-           int(x.dtype == torch.float32),
-           _aligned(C, x, res, gate if mode == 2 else None, du, dh, dx, dres, keep if mode == 2 else None), _nk(post),
-           _nk(pre), mode_b, rpg, float(scale), *d[:5], ptr(d[5]))
+        dgate = torch.empty_like(gate)  # written all the same
+    gp = None if gate is None else gate.data_ptr()
+    dgp = None if dgate is None else dgate.data_ptr()
+    bits = xp | (rp or 0) | (up or 0) | (hp or 0) | (dxp or 0) | (drp or 0)
+    if mode == 2:
+        bits |= gp | dgp
+    hip_on(dev, "ptg_block_norm_bwd", xp, rp, gp, up, hp, dxp, drp, g1, b1, g2, stats.data_ptr(), ptr(vecs[0]),
+           ptr(vecs[1]), ptr(vecs[2]), ptr(vecs[3]), dgp, workspace.data_ptr(), M, C, f32, C % 8 == 0 and not bits & 15,
+           k1, k2, mode, rpg, scale, d[0], d[1], d[2], d[3], d[4], ptr(d[5]))
     return dx, dres
 
 
@@ -238,6 +280,7 @@ _WS: dict = {}
 
 
 def block_norm_workspace_floats(rows: int, cols: int, groups: int) -> int:
+    """Floats of :func:`block_norm_workspace`."""
     key = (rows, cols, groups)
     v = _WS.get(key)
     if v is None:
@@ -249,25 +292,6 @@ def block_norm_workspace_floats(rows: int, cols: int, groups: int) -> int:
             _WS.clear()
         v = _WS[key] = n.value
     return v
-
-
-def _no_overlap(ins, outs, allow):
-    """Outputs must not overlap inputs or one another; a pair in ``allow`` may be the very same buffer
-    (every element is read before it is written, by the same thread)."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
-
-    named = [(n, t) for n, t in ins.items() if t is not None and t.numel()]
-    done = []
-    for on, o in outs.items():
-        if o is None or not o.numel():
-            continue
-        lo, hi = span(o)
-        for n, t in named + done:
-            a, b = span(t)
-            if lo < b and a < hi and not ((n, on) in allow and (a, b) == (lo, hi)):
-                raise ValueError(f"block_norm: {on} overlaps {n}")
-        done.append((on, o))
 
 
 # ---------------------------------------------------------------------------------------- reference
