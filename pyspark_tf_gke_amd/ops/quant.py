@@ -22,7 +22,7 @@ ACT = {None: 0, "linear": 0, "relu": 1}
 
 class Int4Weight(NamedTuple):
     """Laid-out weights: tiles uint8 [N/16, K/128, 64, 16], scale bf16 and zero uint8 (or None)
-    [N/16, K/128, 128/group, 16], sizes rounded up (padding has scale 0)."""
+    [N/16, K/128, 16, 128/group], sizes rounded up (padding has scale 0)."""
 
     tiles: torch.Tensor
     scale: torch.Tensor
@@ -111,7 +111,7 @@ def int4_layout(codes, scale, zero=None, group: int = 128) -> Int4Weight:
             return None
         p = torch.zeros((Np, Kp // group), dtype=t.dtype, device=t.device)
         p[:N, : K // group] = t
-        return p.view(Np // 16, 16, Kp // 128, 128 // group).permute(0, 2, 3, 1).contiguous()
+        return p.view(Np // 16, 16, Kp // 128, 128 // group).permute(0, 2, 1, 3).contiguous()
 
     return Int4Weight(tiles, group_rows(scale), group_rows(zero), N, K, group)
 
@@ -127,7 +127,7 @@ def int4_codes(w: Int4Weight):
     q = ((words[..., None, None] >> sh) & 15).reshape(nt * 16, kt * 128)[: w.n, : w.k].to(torch.uint8)
 
     def rows(t):
-        return None if t is None else t.permute(0, 3, 1, 2).reshape(nt * 16, -1)[: w.n, : w.k // w.group].contiguous()
+        return None if t is None else t.permute(0, 2, 1, 3).reshape(nt * 16, -1)[: w.n, : w.k // w.group].contiguous()
 
     return q[:, 0::2] | (q[:, 1::2] << 4), rows(w.scale), rows(w.zero)
 
