@@ -34,14 +34,55 @@ PTG_DEV U4 dec8(uint32_t w) {
   return o;
 }
 
+// An output again, term by term from the definition.  The offset sums above turn an infinity among the
+// inputs (and a product that leaves fp32 at 31 times its size) into NaN; an output that came out infinite
+// or NaN is settled here, so y is what the formula gives for any x.  Finite outputs never come here.
+template <int GS>
+PTG_DEV float int4_term_by_term(const bf16_t* x, const uint8_t* w, const bf16_t* scale, const uint8_t* zero, int n,
+                                int K, int kt) {
+  float s = 0.f;
+  for (int k = 0; k < K; k += 8) {
+    const long tile = (long)(n >> 4) * kt + k / QT_K;
+    const int i = (k & 127) >> 5, quarter = (k & 31) >> 3;
+    uint32_t d = *(const uint32_t*)(w + tile * 1024 + (quarter * 16 + (n & 15)) * 16 + i * 4);
+    d = __builtin_amdgcn_alignbit(d, d, 3);
+    const long si = (tile * 16 + (n & 15)) * (4 / GS) + i / GS;
+    const float sc = bf2f(scale[si]), z = zero ? (float)zero[si] : 8.f;
+    for (int e = 0; e < 8; ++e)
+      s = fmaf(((float)((d >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - z) * sc, bf2f(x[k + e]), s);
+    if (s != s) break;
+  }
+  return s;
+}
+struct Args4 {
+  const bf16_t* x;
+  const uint8_t* w;
+  const bf16_t* s;
+  const uint8_t* z;
+  const float* b;
+  void* y;
+  float* part;  // null: the kernel finishes y itself
+  int M, N, K, kt, act, f32;
+};
+// y[m][n] from the sum s over all of K
+template <int GS>
+PTG_DEV void int4_finish(const Args4& a, int m, int n, float s) {
+  if (!(fabsf(s) < __builtin_inff())) s = int4_term_by_term<GS>(a.x + (long)m * a.K, a.w, a.s, a.z, n, a.K, a.kt);
+  if (a.b) s += a.b[n];
+  if (a.act && s < 0.f) s = 0.f;  // NaN stays
+  const long o = (long)m * a.N + n;
+  if (a.f32) ((float*)a.y)[o] = s;
+  else ((bf16_t*)a.y)[o] = f2bf(s);
+}
+
 }  // namespace
 
 // A wave computes 16 * MT rows x 16 * NT outputs over its share of K; the NW waves of a workgroup take the
 // tiles of the workgroup's K range in turn and are joined in LDS in a fixed order.  One wave is one MFMA
 // chain a product tile: sum (16 + u) x on top of -(16 + z) * sum x, the latter from one MFMA with ones for
 // every 32 inputs that all NT tiles share.  The next tile's weights, scales and inputs are loaded before
-// the current tile is worked on.  part == nullptr: the range is all of K and the workgroup finishes y
-// itself; otherwise it leaves fp32 sums in part[split][M][N].
+// the current tile is worked on.  Where K is split
+// over workgroups they leave fp32 sums in part[split][M][N], else they finish y.
 template <int GS>
 struct Group {  // of a tile: 4 / GS groups
   static constexpr int NG = 4 / GS;
@@ -49,16 +90,17 @@ struct Group {  // of a tile: 4 / GS groups
   uint8_t z[NG];
 };
 template <int MT, int NT, int NW, int GS, bool HASZ>
-__global__ __launch_bounds__(NW * 64) void int4_mm_k(const bf16_t* __restrict__ x, const uint8_t* __restrict__ w,
-                                                     const bf16_t* __restrict__ scale,
-                                                     const uint8_t* __restrict__ zero, const float* __restrict__ bias,
-                                                     void* __restrict__ y, float* __restrict__ part, int M, int N,
-                                                     int K, int kt, int act, int f32) {
+__global__ __launch_bounds__(NW * 64) void int4_mm_k(Args4 a) {
   constexpr int NG = 4 / GS, R = MT * NT * 4;
   constexpr bool FLAT = R * NW <= 128;  // every wave's sums in LDS at once, else pairwise
   __shared__ float red[(FLAT ? NW : NW / 2) * R][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, q = lane >> 4;
   const int sp = blockIdx.x, splits = gridDim.x, nb = blockIdx.y * NT, m0 = blockIdx.z * 16 * MT;
+  const int M = a.M, N = a.N, K = a.K, kt = a.kt;
+  const bf16_t* __restrict__ x = a.x;
+  const uint8_t* __restrict__ w = a.w;
+  const bf16_t* __restrict__ scale = a.s;
+  const uint8_t* __restrict__ zero = a.z;
   const int ntiles = (N + 15) / 16;
   const int t0 = (int)((long)kt * sp / splits), t1 = (int)((long)kt * (sp + 1) / splits);
   const bf16_t* xr[MT];
@@ -147,15 +189,8 @@ __global__ __launch_bounds__(NW * 64) void int4_mm_k(const bf16_t* __restrict__ 
     const int i = v / (NT * 4), n = (v / 4) % NT, r = v & 3;
     const int col = (nb + n) * 16 + (l & 15), m = m0 + i * 16 + (l >> 4) * 4 + r;
     if (m >= M || col >= N) return;
-    const long o = (long)m * N + col;
-    if (part) {
-      part[(long)sp * M * N + o] = s;
-      return;
-    }
-    if (bias) s += bias[col];
-    if (act) s = fmaxf(s, 0.f);
-    if (f32) ((float*)y)[o] = s;
-    else ((bf16_t*)y)[o] = f2bf(s);
+    if (a.part) a.part[((long)sp * M + m) * N + col] = s;
+    else int4_finish<GS>(a, m, col, s);
   };
   if (FLAT) {
     put(wave);
@@ -192,63 +227,232 @@ __global__ __launch_bounds__(NW * 64) void int4_mm_k(const bf16_t* __restrict__ 
   }
 }
 
-// y = act(sum of the splits + bias)
-template <bool F32>
-__global__ __launch_bounds__(256) void int4_join_k(const float* __restrict__ part, const float* __restrict__ bias,
-                                                   void* __restrict__ y, long total, int N, int splits, int act) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+// Batches of more than 32 rows are bound by the matrix cores and by what feeds them, not by HBM: a
+// workgroup of WM x WN waves takes 64 * WM rows x 64 * WN outputs, each wave 64 x 64 of them, and stages
+// inputs and weights of 128 inputs at a time in a ring of NS LDS buffers by direct loads (no registers),
+// NS - 1 stages ahead.  Inputs lie in LDS as rows of 16 chunks of 16 bytes, chunk c of row r at place
+// c ^ (r & 15): the 16 rows that a wave reads at once are in 16 places, free of bank conflicts.  Weights
+// stay in 4 bits until a wave has them in registers.
+template <int WM, int WN, int NS>
+struct Tile4 {
+  static constexpr int XB = WM * 64 * 256, WB = WN * 4 * 1024, STAGE = XB + WB;
+  static constexpr int XL = 16 / WN, WL = 4 / WM, L = XL + WL;  // loads of a wave a stage
+  static constexpr int LDS = NS * STAGE;
+};
+typedef __attribute__((address_space(3))) void q_lds_t;
+template <int N>
+PTG_DEV void q_wait_vm() {  // at most N vector loads in flight, no LDS read
+  static_assert(N >= 0 && N < 64, "vmcnt");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | ((N >> 4) << 14));
+}
+template <int WM, int WN, int NS, int GS, bool HASZ>
+__global__ __launch_bounds__(WM* WN * 64) void int4_tile_k(Args4 a, int mb, int nbk, int splits) {
+  using T = Tile4<WM, WN, NS>;
+  constexpr int NG = 4 / GS, NW = WM * WN;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, q = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wid / WN, wn = wid % WN;
+  // the tiles of one split are neighbours on one XCD: its L2 reads that split's inputs and weights once
+  const int item = xcd_remap(blockIdx.x, gridDim.x), sp = item / (mb * nbk), rest = item - sp * (mb * nbk);
+  const int m0 = (rest % mb) * 64 * WM, nb = (rest / mb) * 4 * WN, ntiles = (a.N + 15) / 16, kt = a.kt;
+  const int t0 = (int)((long)kt * sp / splits), nk = (int)((long)kt * (sp + 1) / splits) - t0;
+  const Rsrc rx = make_rsrc(a.x + (long)m0 * a.K, (uint32_t)min(a.M - m0, 64 * WM) * (uint32_t)a.K * 2u);
+  const Rsrc rw = make_rsrc(a.w + (long)nb * kt * 1024, (uint32_t)min(ntiles - nb, 4 * WN) * (uint32_t)kt * 1024u);
+  uint32_t xo[T::XL], wo[T::WL];
+  int xk[T::XL];
+#pragma unroll
+  for (int j = 0; j < T::XL; ++j) {  // 4 rows a load
+    const int row = (wid * T::XL + j) * 4 + q, chunk = n16 ^ (row & 15);
+    xk[j] = t0 * QT_K + chunk * 8;
+    xo[j] = ((uint32_t)row * (uint32_t)a.K + (uint32_t)xk[j]) * 2u;
+  }
+#pragma unroll
+  for (int j = 0; j < T::WL; ++j)
+    wo[j] = ((uint32_t)(wid * T::WL + j) * (uint32_t)kt + (uint32_t)t0) * 1024u + (uint32_t)lane * 16u;
+  // stages past the end are issued too, out of range (zeros, no traffic): the count of loads in flight stays known
+  auto issue = [&](int t) {
+    unsigned char* base = smem + (t % NS) * T::STAGE;
+    const bool live = t < nk;
+#pragma unroll
+    for (int j = 0; j < T::XL; ++j) {
+      const uint32_t o = live && xk[j] + t * QT_K < a.K ? xo[j] + (uint32_t)t * (QT_K * 2u) : PTG_OOB;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (q_lds_t*)(base + (wid * T::XL + j) * 1024), 16, o, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < T::WL; ++j) {
+      const uint32_t o = live ? wo[j] + (uint32_t)t * 1024u : PTG_OOB;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (q_lds_t*)(base + T::XB + (wid * T::WL + j) * 1024), 16, o, 0, 0, 0);
+    }
+  };
+  long gi[4];  // where this lane's scales of a tile of outputs start
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int nt = nb + wn * 4 + n;
+    gi[n] = ((long)(nt < ntiles ? nt : ntiles - 1) * kt + t0) * 16 + n16;
+  }
+  Group<GS> gn[4];
+  auto scales = [&](int t) {
+    t = t < nk ? t : nk - 1;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const long at = (gi[n] + t * 16) * NG;
+      __builtin_memcpy(gn[n].s, a.s + at, 2 * NG);
+      if (HASZ) __builtin_memcpy(gn[n].z, a.z + at, NG);
+    }
+  };
+  f32x4_t acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) acc[i][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  U4 ones;
+  ones.x = 0x3F803F80u; ones.y = ones.x; ones.z = ones.x; ones.w = ones.x;
+  scales(0);
+#pragma unroll
+  for (int t = 0; t < NS - 1; ++t) issue(t);
+  for (int t = 0; t < nk; ++t) {
+    q_wait_vm<T::L*(NS - 2)>();    // this wave's part of stage t has landed
+    __builtin_amdgcn_s_barrier();  // and every wave's; all have left the buffer of stage t - 1
+    asm volatile("" ::: "memory");
+    Group<GS> gc[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) gc[n] = gn[n];
+    scales(t + 1);
+    issue(t + NS - 1);
+    const unsigned char* sx = smem + (t % NS) * T::STAGE + (wm * 64 + n16) * 256;
+    const unsigned char* sw = smem + (t % NS) * T::STAGE + T::XB + wn * 4096 + lane * 16;
+    U4 wv[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) wv[n] = *(const U4*)(sw + n * 1024);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      U4 xa[4][GS];
+      f32x4_t xs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        xs[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < GS; ++j) {
+          xa[i][j] = *(const U4*)(sx + i * 4096 + (((g * GS + j) * 4 + q) ^ n16) * 16);
+          xs[i] = mfma32(xa[i][j], ones, xs[i]);
+        }
+        if (!HASZ) xs[i] *= -24.f;
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint32_t ww[4] = {wv[n].x, wv[n].y, wv[n].z, wv[n].w};
+        const float s = bf2f(gc[n].s[g]);
+        U4 b[GS];
+#pragma unroll
+        for (int j = 0; j < GS; ++j) b[j] = dec8(ww[g * GS + j]);
+        f32x4_t d[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = HASZ ? xs[i] * (-16.f - (float)gc[n].z[g]) : xs[i];
+#pragma unroll
+        for (int j = 0; j < GS; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[i] = mfma32(xa[i][j], b[j], d[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i][n] += d[i] * s;
+      }
+    }
+  }
+  q_wait_vm<0>();
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int m = m0 + wm * 64 + i * 16 + q * 4 + r, col = (nb + wn * 4 + n) * 16 + n16;
+        if (m < a.M && col < a.N) {
+          if (a.part) a.part[((long)sp * a.M + m) * a.N + col] = acc[i][n][r];
+          else int4_finish<GS>(a, m, col, acc[i][n][r]);
+        }
+      }
+}
+
+// y = act(sum of the splits + bias), V outputs of a row a thread
+template <int GS, int V>
+__global__ __launch_bounds__(256) void int4_join_k(Args4 a, int splits) {
+  const long total = (long)a.M * a.N, i = ((long)blockIdx.x * 256 + threadIdx.x) * V;
   if (i >= total) return;
-  float s = 0.f;
-  for (int k = 0; k < splits; ++k) s += part[(long)k * total + i];
-  if (bias) s += bias[i % N];
-  if (act) s = fmaxf(s, 0.f);
-  if (F32) ((float*)y)[i] = s;
-  else ((bf16_t*)y)[i] = f2bf(s);
+  float s[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k) {
+    float p[V];
+    __builtin_memcpy(p, a.part + k * total + i, 4 * V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] += p[j];
+  }
+  const int m = (int)(i / a.N), n = (int)(i - (long)m * a.N);
+#pragma unroll
+  for (int j = 0; j < V; ++j) int4_finish<GS>(a, m, n + j, s[j]);
 }
 
 namespace {
 // Workgroups wanted: one a CU.  Two a CU measured 104.7 against 94.1 us on 256 x 2048 x 20480 and 18.4
 // against 14.2 us on 16 x 8192 x 8192 (more partial sums to write and join); 1 x 2048 x 20480 is the same.
 constexpr int Q_WGS = 256;
-struct Plan4 { int mt, nt, mb, nb, splits; };
-Plan4 plan4(int M, int N, int K) {
+struct Plan4 { int tile, mt, nt, mb, nb, splits; };
+Plan4 plan4(int M, int N, int K, bool aligned) {
   Plan4 p;
-  p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  p.nt = M <= 8 ? 1 : M <= 32 ? 2 : 4;
-  p.mb = (M + 16 * p.mt - 1) / (16 * p.mt);
-  p.nb = (N + 16 * p.nt - 1) / (16 * p.nt);
-  const long wgs = (long)p.nb * p.mb, kt = (K + QT_K - 1) / QT_K;
-  const int nw = p.mt == 1 ? 16 : 8;
+  const long kt = (K + QT_K - 1) / QT_K;
+  p.tile = aligned && M > 32;
+  long least;  // tiles of a split at least
+  if (p.tile) {
+    p.mt = M <= 64 ? 1 : 2;
+    p.nt = 4;
+    p.mb = (M + 64 * p.mt - 1) / (64 * p.mt);
+    p.nb = (N + 64 * p.nt - 1) / (64 * p.nt);
+    least = 4;
+  } else {
+    p.mt = M <= 16 ? 1 : 2;
+    p.nt = M <= 8 ? 1 : 2;
+    p.mb = (M + 16 * p.mt - 1) / (16 * p.mt);
+    p.nb = (N + 16 * p.nt - 1) / (16 * p.nt);
+    least = 2 * (p.mt == 1 ? 16 : 8);  // two a wave
+  }
+  const long wgs = (long)p.nb * p.mb;
   long s = (Q_WGS + wgs - 1) / wgs;
-  if (s > kt / (2 * nw)) s = kt / (2 * nw);  // at least two tiles a wave
+  if (p.tile) s = Q_WGS / wgs;
+  if (s > kt / least) s = kt / least;
   p.splits = s < 1 ? 1 : (int)s;
   return p;
 }
-struct Args4 {
-  const bf16_t* x;
-  const uint8_t* w;
-  const bf16_t* s;
-  const uint8_t* z;
-  const float* b;
-  void* y;
-  float* part;
-  int M, N, K, act, f32;
-  hipStream_t st;
-};
 template <int MT, int NT, int NW, int GS>
-void go4z(const Plan4& p, const Args4& a) {
-  const int kt = (a.K + QT_K - 1) / QT_K;
+void go4(const Plan4& p, const Args4& a, hipStream_t st) {
   const dim3 grid(p.splits, p.nb, p.mb);
-  if (a.z)
-    int4_mm_k<MT, NT, NW, GS, true><<<grid, NW * 64, 0, a.st>>>(a.x, a.w, a.s, a.z, a.b, a.y, a.part, a.M, a.N, a.K, kt, a.act, a.f32);
-  else
-    int4_mm_k<MT, NT, NW, GS, false><<<grid, NW * 64, 0, a.st>>>(a.x, a.w, a.s, a.z, a.b, a.y, a.part, a.M, a.N, a.K, kt, a.act, a.f32);
+  if (a.z) int4_mm_k<MT, NT, NW, GS, true><<<grid, NW * 64, 0, st>>>(a);
+  else int4_mm_k<MT, NT, NW, GS, false><<<grid, NW * 64, 0, st>>>(a);
 }
-template <int MT, int NT, int NW>
-void go4(int gs, const Plan4& p, const Args4& a) {
-  if (gs == 1) go4z<MT, NT, NW, 1>(p, a);
-  else if (gs == 2) go4z<MT, NT, NW, 2>(p, a);
-  else go4z<MT, NT, NW, 4>(p, a);
+template <int WM, int WN, int NS, int GS>
+void go4t(const Plan4& p, const Args4& a, hipStream_t st) {
+  auto kern = a.z ? int4_tile_k<WM, WN, NS, GS, true> : int4_tile_k<WM, WN, NS, GS, false>;
+  constexpr int lds = Tile4<WM, WN, NS>::LDS;
+  static bool set[2];  // per kernel; setting it twice is harmless
+  if (!set[a.z != nullptr]) {
+    (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    set[a.z != nullptr] = true;
+  }
+  kern<<<p.mb * p.nb * p.splits, WM * WN * 64, lds, st>>>(a, p.mb, p.nb, p.splits);
+}
+template <int GS>
+int go4g(const Plan4& p, const Args4& a, hipStream_t st) {
+  if (p.tile && p.mt == 1) go4t<1, 4, 3, GS>(p, a, st);
+  else if (p.tile) go4t<2, 4, 3, GS>(p, a, st);
+  else if (p.mt == 1 && p.nt == 1) go4<1, 1, 16, GS>(p, a, st);
+  else if (p.mt == 1) go4<1, 2, 16, GS>(p, a, st);
+  else go4<2, 2, 8, GS>(p, a, st);
+  if (a.part) {
+    const long total = (long)a.M * a.N;
+    if (a.N % 4 == 0) int4_join_k<GS, 4><<<(int)((total / 4 + 255) / 256), 256, 0, st>>>(a, p.splits);
+    else int4_join_k<GS, 1><<<(int)((total + 255) / 256), 256, 0, st>>>(a, p.splits);
+  }
+  PTG_RETURN_LAUNCH();
 }
 }  // namespace
 
@@ -256,8 +460,12 @@ extern "C" {
 
 // *floats: workspace of a product of M rows (0 where none is needed)
 int ptg_int4_ws(int M, int N, int K, void* floats) {
-  const Plan4 p = M > 0 ? plan4(M, N, K) : Plan4{1, 1, 1, 1, 1};
-  *(long*)floats = p.splits > 1 ? (long)p.splits * M * N : 0;
+  long most = 0;
+  for (int al = 0; al < 2 && M > 0; ++al) {
+    const Plan4 p = plan4(M, N, K, al != 0);
+    if (p.splits > 1 && p.splits > most) most = p.splits;
+  }
+  *(long*)floats = most * M * N;
   return 0;
 }
 
@@ -265,23 +473,16 @@ int ptg_int4_ws(int M, int N, int K, void* floats) {
 int ptg_int4_dense(const void* x, const void* w, const void* scale, const void* zero, const void* bias, void* y,
                    void* ws, int M, int N, int K, int group, int act, int f32, hipStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
-  if ((group != 32 && group != 64 && group != 128) || K < group || K % group) return (int)hipErrorInvalidValue;
-  const Plan4 p = plan4(M, N, K);
-  float* part = p.splits > 1 ? (float*)ws : nullptr;
-  const Args4 a{(const bf16_t*)x, (const uint8_t*)w, (const bf16_t*)scale, (const uint8_t*)zero, (const float*)bias, y,
-                part, M, N, K, act, f32, stream};
-  const int gs = group / 32;
-  if (p.mt == 1 && p.nt == 1) go4<1, 1, 16>(gs, p, a);
-  else if (p.mt == 1) go4<1, 2, 16>(gs, p, a);
-  else if (p.mt == 2) go4<2, 2, 8>(gs, p, a);
-  else go4<4, 4, 8>(gs, p, a);
-  if (part) {
-    const long total = (long)M * N;
-    const int blocks = (int)((total + 255) / 256);
-    if (f32) int4_join_k<true><<<blocks, 256, 0, stream>>>(part, (const float*)bias, y, total, N, p.splits, act);
-    else int4_join_k<false><<<blocks, 256, 0, stream>>>(part, (const float*)bias, y, total, N, p.splits, act);
-  }
-  PTG_RETURN_LAUNCH();
+  // a block of rows or of outputs stays below 2 GiB
+  if ((group != 32 && group != 64 && group != 128) || K < group || K % group || K > (1 << 22))
+    return (int)hipErrorInvalidValue;
+  const Plan4 p = plan4(M, N, K, ((uintptr_t)x & 15) == 0);
+  if (p.splits > 1 && !ws) return (int)hipErrorInvalidValue;
+  const Args4 a{(const bf16_t*)x, (const uint8_t*)w, (const bf16_t*)scale, (const uint8_t*)zero, (const float*)bias,
+                y, p.splits > 1 ? (float*)ws : nullptr, M, N, K, (K + QT_K - 1) / QT_K, act, f32};
+  if (group == 32) return go4g<1>(p, a, stream);
+  if (group == 64) return go4g<2>(p, a, stream);
+  return go4g<4>(p, a, stream);
 }
 
 }  // extern "C"

@@ -16,7 +16,8 @@ def weights64(codes, scale, zero, group):
 
 SHAPES = [(1, 1, 32, 32), (1, 16, 128, 128), (3, 17, 160, 32), (5, 33, 320, 64), (16, 100, 1024, 128),
           (17, 48, 2048, 64), (1, 2048, 20480, 128), (2, 7, 4096, 32), (33, 130, 1280, 128), (64, 64, 512, 64),
-          (65, 50, 1056, 32), (130, 300, 2560, 128), (256, 64, 640, 64), (300, 272, 1152, 128), (1, 5000, 256, 64)]
+          (65, 50, 1056, 32), (130, 300, 2560, 128), (256, 64, 640, 64), (300, 272, 1152, 128), (1, 5000, 256, 64),
+          (70, 530, 3040, 32), (40, 256, 20480, 64), (129, 1000, 4160, 64)]
 
 
 @pytest.mark.parametrize("B,N,K,group", SHAPES)
@@ -76,12 +77,53 @@ def test_rows_do_not_mix_and_nothing_else_is_written(hip_built):
     Q.int4_dense_fwd(x[:0], w, None, None, out[:0])
 
 
-def test_unaligned_input(hip_built):
+@pytest.mark.parametrize("B,N,K,group", [(3, 20, 160, 32), (66, 20, 160, 32), (40, 300, 1088, 64), (12, 20, 192, 64)])
+def test_padding_reads_nothing_of_a_neighbour(hip_built, B, N, K, group):
+    """K % 128 != 0: the tile's rest lies over the next row, here all NaN; the last row's over NaN too."""
+    codes, scale, z, _ = codes_for(N, K, group, True, dev="cuda")
+    w = Q.int4_layout(codes, scale, z, group)
+    buf = torch.full((2 * B + 1, K), float("nan"), device="cuda", dtype=torch.bfloat16)
+    x = torch.randint(-1, 2, (B, K), device="cuda").to(torch.bfloat16)
+    buf[:B] = x
+    buf[1:B:2] = float("nan")
+    out = torch.empty(B, N, device="cuda")
+    Q.int4_dense_fwd(buf[:B], w, None, None, out)
+    want = x.double() @ weights64(codes, scale, z, group).t()
+    assert torch.equal(out[0::2].double(), want[0::2]) and torch.isnan(out[1::2]).all()
+
+
+@pytest.mark.parametrize("B,N,K,group", [(1, 40, 4096, 128), (16, 33, 256, 32), (30, 20, 512, 64), (70, 300, 8192, 128)])
+@pytest.mark.parametrize("zero", [False, True])
+def test_infinities_and_large_inputs(hip_built, B, N, K, group, zero):
+    """Row 0 has one infinity, row 1 two of one sign, row 2 a NaN, row 3 values near the largest number that
+    cancel: the outputs are those of the formula, and ReLU keeps a NaN."""
+    codes, scale, z, _ = codes_for(N, K, group, zero, dev="cuda")
+    w = Q.int4_layout(codes, scale, z, group)
+    x = torch.randint(-1, 2, (B, K), device="cuda").to(torch.bfloat16)
+    x[0, 5] = float("inf")
+    if B > 3:
+        x[1, 3], x[1, K - 1] = float("-inf"), float("-inf")
+        x[2, 7] = float("nan")
+        x[3] = 0
+        x[3, 0] = 2.0**125
+    out, pos = torch.empty(B, N, device="cuda"), torch.empty(B, N, device="cuda")
+    Q.int4_dense_fwd(x, w, None, None, out)
+    Q.int4_dense_fwd(x, w, None, "relu", pos)
+    w64 = weights64(codes, scale, z, group)
+    want = (x.double()[:, None] * w64[None]).sum(2).float()  # single terms, no offset
+    assert torch.isinf(want[0]).any()
+    assert torch.equal(torch.nan_to_num(out, nan=7.0), torch.nan_to_num(want, nan=7.0))
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(pos, nan=7.0), torch.nan_to_num(torch.relu(want), nan=7.0))
+
+
+@pytest.mark.parametrize("B", [4, 20, 70])
+def test_unaligned_input(hip_built, B):
     codes, scale, z, _ = codes_for(40, 256, 64, True, dev="cuda")
     w = Q.int4_layout(codes, scale, z, 64)
-    b = torch.randint(-1, 2, (4 * 256 + 1,), device="cuda").to(torch.bfloat16)
-    x = b[1:].view(4, 256)
-    out, want = torch.empty(4, 40, device="cuda"), torch.empty(4, 40, device="cuda")
+    b = torch.randint(-1, 2, (B * 256 + 1,), device="cuda").to(torch.bfloat16)
+    x = b[1:].view(B, 256)
+    out, want = torch.empty(B, 40, device="cuda"), torch.empty(B, 40, device="cuda")
     Q.int4_dense_fwd(x, w, None, None, out)
     Q.int4_dense_fwd(x.clone(), w, None, None, want)
     assert torch.equal(out, want)
