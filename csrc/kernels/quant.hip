@@ -24,8 +24,8 @@ PTG_DEV f32x4_t mfma32(const U4& a, const U4& b, f32x4_t c) {
                                                  0, 0, 0);
 }
 // 8 weights of a dword as bf16 16 + u
-PTG_DEV U4 dec8(uint32_t w) {
-  constexpr uint32_t M = 0x00780078u, E = 0x41804180u;
+PTG_DEV U4 dec8(uint32_t w, uint32_t E = 0x41804180u) {
+  constexpr uint32_t M = 0x00780078u;
   U4 o;
   o.x = (w & M) | E;
   o.y = ((w >> 4) & M) | E;
@@ -227,18 +227,13 @@ __global__ __launch_bounds__(NW * 64) void int4_mm_k(Args4 a) {
   }
 }
 
-// Batches of more than 32 rows are bound by the matrix cores and by what feeds them, not by HBM: a
-// workgroup of WM x WN waves takes 64 * WM rows x 64 * WN outputs, each wave 64 x 64 of them, and stages
-// inputs and weights of 128 inputs at a time in a ring of NS LDS buffers by direct loads (no registers),
-// NS - 1 stages ahead.  Inputs lie in LDS as rows of 16 chunks of 16 bytes, chunk c of row r at place
-// c ^ (r & 15): the 16 rows that a wave reads at once are in 16 places, free of bank conflicts.  Weights
-// stay in 4 bits until a wave has them in registers.
-template <int WM, int WN, int NS>
-struct Tile4 {
-  static constexpr int XB = WM * 64 * 256, WB = WN * 4 * 1024, STAGE = XB + WB;
-  static constexpr int XL = 16 / WN, WL = 4 / WM, L = XL + WL;  // loads of a wave a stage
-  static constexpr int LDS = NS * STAGE;
-};
+// Batches of more than 32 rows are bound by the matrix cores and by what feeds them, not by HBM.  A workgroup
+// takes 64 rows x 256 outputs; 4 waves hold 64 x 64 of them each, twice over: waves 4..7 work on every
+// other stage of 128 inputs, so two waves share a SIMD and one multiplies while the other waits, and the
+// two halves are added at the end.  A stage (64 rows of inputs, 16 KB, and 16 weight tiles, 16 KB) goes
+// straight to LDS, into a ring of QR.  Inputs lie there as rows of 16 chunks of 16 bytes, chunk c of row
+// r at place c ^ (r & 15): the 16 rows that a wave reads at once are in 16 places, free of bank conflicts.
+constexpr int QT_M = 64, QT_N = 256, QR = 5, Q_XB = QT_M * 256, Q_STAGE = Q_XB + QT_N / 16 * 1024;
 typedef __attribute__((address_space(3))) void q_lds_t;
 template <int N>
 PTG_DEV void q_wait_vm() {  // at most N vector loads in flight, no LDS read
@@ -246,59 +241,56 @@ PTG_DEV void q_wait_vm() {  // at most N vector loads in flight, no LDS read
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | ((N >> 4) << 14));
 }
-template <int WM, int WN, int NS, int GS, bool HASZ>
-__global__ __launch_bounds__(WM* WN * 64) void int4_tile_k(Args4 a, int mb, int nbk, int splits) {
-  using T = Tile4<WM, WN, NS>;
-  constexpr int NG = 4 / GS, NW = WM * WN;
+template <int GS, bool HASZ>
+__global__ __launch_bounds__(512) void int4_tile_k(Args4 a, int mb, int nbk, int splits) {
+  constexpr int NG = 4 / GS;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, q = lane >> 4;
-  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wid / WN, wn = wid % WN;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), half = wid >> 2, wn = wid & 3;
   // the tiles of one split are neighbours on one XCD: its L2 reads that split's inputs and weights once
   const int item = xcd_remap(blockIdx.x, gridDim.x), sp = item / (mb * nbk), rest = item - sp * (mb * nbk);
-  const int m0 = (rest % mb) * 64 * WM, nb = (rest / mb) * 4 * WN, ntiles = (a.N + 15) / 16, kt = a.kt;
+  const int m0 = (rest % mb) * QT_M, nb = (rest / mb) * (QT_N / 16), ntiles = (a.N + 15) / 16, kt = a.kt;
   const int t0 = (int)((long)kt * sp / splits), nk = (int)((long)kt * (sp + 1) / splits) - t0;
-  const Rsrc rx = make_rsrc(a.x + (long)m0 * a.K, (uint32_t)min(a.M - m0, 64 * WM) * (uint32_t)a.K * 2u);
-  const Rsrc rw = make_rsrc(a.w + (long)nb * kt * 1024, (uint32_t)min(ntiles - nb, 4 * WN) * (uint32_t)kt * 1024u);
-  uint32_t xo[T::XL], wo[T::WL];
-  int xk[T::XL];
+  const Rsrc rx = make_rsrc(a.x + (long)m0 * a.K, (uint32_t)min(a.M - m0, QT_M) * (uint32_t)a.K * 2u);
+  const Rsrc rw = make_rsrc(a.w + (long)nb * kt * 1024, (uint32_t)min(ntiles - nb, QT_N / 16) * (uint32_t)kt * 1024u);
+  // a wave loads 8 rows of inputs (4 at a time) and 2 weight tiles of each stage
+  uint32_t xo[2], wo[2];
+  int xt[2];  // stages whose chunk exists
 #pragma unroll
-  for (int j = 0; j < T::XL; ++j) {  // 4 rows a load
-    const int row = (wid * T::XL + j) * 4 + q, chunk = n16 ^ (row & 15);
-    xk[j] = t0 * QT_K + chunk * 8;
-    xo[j] = ((uint32_t)row * (uint32_t)a.K + (uint32_t)xk[j]) * 2u;
+  for (int j = 0; j < 2; ++j) {
+    const int row = (wid * 2 + j) * 4 + q, k = t0 * QT_K + (n16 ^ (row & 15)) * 8;
+    xo[j] = ((uint32_t)row * (uint32_t)a.K + (uint32_t)k) * 2u;
+    xt[j] = min(nk, (a.K - k + QT_K - 1) / QT_K);
+    wo[j] = ((uint32_t)(wid * 2 + j) * (uint32_t)kt + (uint32_t)t0) * 1024u + (uint32_t)lane * 16u;
   }
-#pragma unroll
-  for (int j = 0; j < T::WL; ++j)
-    wo[j] = ((uint32_t)(wid * T::WL + j) * (uint32_t)kt + (uint32_t)t0) * 1024u + (uint32_t)lane * 16u;
   // stages past the end are issued too, out of range (zeros, no traffic): the count of loads in flight stays known
-  auto issue = [&](int t) {
-    unsigned char* base = smem + (t % NS) * T::STAGE;
-    const bool live = t < nk;
+  auto issue = [&](int t, int slot) {
+    unsigned char* base = smem + slot * Q_STAGE + wid * 2048;
 #pragma unroll
-    for (int j = 0; j < T::XL; ++j) {
-      const uint32_t o = live && xk[j] + t * QT_K < a.K ? xo[j] + (uint32_t)t * (QT_K * 2u) : PTG_OOB;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (q_lds_t*)(base + (wid * T::XL + j) * 1024), 16, o, 0, 0, 0);
-    }
+    for (int j = 0; j < 2; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (q_lds_t*)(base + j * 1024), 16,
+                                               t < xt[j] ? xo[j] + (uint32_t)t * (QT_K * 2u) : PTG_OOB, 0, 0, 0);
+    const uint32_t wt = t < nk ? (uint32_t)t * 1024u : PTG_OOB;
 #pragma unroll
-    for (int j = 0; j < T::WL; ++j) {
-      const uint32_t o = live ? wo[j] + (uint32_t)t * 1024u : PTG_OOB;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (q_lds_t*)(base + T::XB + (wid * T::WL + j) * 1024), 16, o, 0, 0, 0);
-    }
+    for (int j = 0; j < 2; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (q_lds_t*)(base + Q_XB + j * 1024), 16, wo[j] + wt, 0, 0, 0);
   };
-  long gi[4];  // where this lane's scales of a tile of outputs start
+  const bf16_t* sp_[4];  // this lane's scales and zero points of the next stage
+  const uint8_t* zp_[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
     const int nt = nb + wn * 4 + n;
-    gi[n] = ((long)(nt < ntiles ? nt : ntiles - 1) * kt + t0) * 16 + n16;
+    const long at = (((long)(nt < ntiles ? nt : ntiles - 1) * kt + t0) * 16 + n16) * NG;
+    sp_[n] = a.s + at;
+    if (HASZ) zp_[n] = a.z + at;
   }
   Group<GS> gn[4];
   auto scales = [&](int t) {
     t = t < nk ? t : nk - 1;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      const long at = (gi[n] + t * 16) * NG;
-      __builtin_memcpy(gn[n].s, a.s + at, 2 * NG);
-      if (HASZ) __builtin_memcpy(gn[n].z, a.z + at, NG);
+      __builtin_memcpy(gn[n].s, sp_[n] + t * 16 * NG, 2 * NG);
+      if (HASZ) __builtin_memcpy(gn[n].z, zp_[n] + t * 16 * NG, NG);
     }
   };
   f32x4_t acc[4][4];
@@ -308,69 +300,92 @@ __global__ __launch_bounds__(WM* WN * 64) void int4_tile_k(Args4 a, int mb, int 
     for (int n = 0; n < 4; ++n) acc[i][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   U4 ones;
   ones.x = 0x3F803F80u; ones.y = ones.x; ones.z = ones.x; ones.w = ones.x;
-  scales(0);
+  uint32_t e16 = 0x41804180u;
+  asm volatile("" : "+v"(e16));  // in a vector register: and-or takes one scalar
+  scales(half);
 #pragma unroll
-  for (int t = 0; t < NS - 1; ++t) issue(t);
-  for (int t = 0; t < nk; ++t) {
-    q_wait_vm<T::L*(NS - 2)>();    // this wave's part of stage t has landed
-    __builtin_amdgcn_s_barrier();  // and every wave's; all have left the buffer of stage t - 1
+  for (int t = 0; t < QR - 2; ++t) issue(t, t);
+  int slot = 0, free = QR - 2;  // of stage t; of stage t + QR - 2
+  for (int t = 0; t < nk; t += 2) {
+    q_wait_vm<4 * (QR - 4)>();     // this wave's part of stages t and t + 1 has landed
+    __builtin_amdgcn_s_barrier();  // and every wave's; all have left the buffers of the two before
     asm volatile("" ::: "memory");
     Group<GS> gc[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) gc[n] = gn[n];
-    scales(t + 1);
-    issue(t + NS - 1);
-    const unsigned char* sx = smem + (t % NS) * T::STAGE + (wm * 64 + n16) * 256;
-    const unsigned char* sw = smem + (t % NS) * T::STAGE + T::XB + wn * 4096 + lane * 16;
+    scales(t + 2 + half);
+    issue(t + QR - 2, free);
+    free = free + 1 == QR ? 0 : free + 1;
+    issue(t + QR - 1, free);
+    free = free + 1 == QR ? 0 : free + 1;
+    const int other = slot + 1 == QR ? 0 : slot + 1;
+    const unsigned char* st = smem + (half ? other : slot) * Q_STAGE;
+    slot = other + 1 == QR ? 0 : other + 1;
+    const unsigned char* sx = st + n16 * 256;
     U4 wv[4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) wv[n] = *(const U4*)(sw + n * 1024);
+    for (int n = 0; n < 4; ++n) wv[n] = *(const U4*)(st + Q_XB + wn * 4096 + lane * 16 + n * 1024);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      U4 xa[4][GS];
-      f32x4_t xs[4];
+      f32x4_t xs[4], d[4][4];
+      const f32x4_t z4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        xs[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < GS; ++j) {
+        const int jj = g * GS + j;
+        U4 x[4];
 #pragma unroll
-        for (int j = 0; j < GS; ++j) {
-          xa[i][j] = *(const U4*)(sx + i * 4096 + (((g * GS + j) * 4 + q) ^ n16) * 16);
-          xs[i] = mfma32(xa[i][j], ones, xs[i]);
+        for (int i = 0; i < 4; ++i) x[i] = *(const U4*)(sx + i * 4096 + ((jj * 4 + q) ^ n16) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xs[i] = mfma32(x[i], ones, j ? xs[i] : z4);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t ww[4] = {wv[n].x, wv[n].y, wv[n].z, wv[n].w};
+          const U4 b = dec8(ww[jj], e16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[i][n] = mfma32(x[i], b, j ? d[i][n] : z4);
         }
-        if (!HASZ) xs[i] *= -24.f;
       }
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const uint32_t ww[4] = {wv[n].x, wv[n].y, wv[n].z, wv[n].w};
-        const float s = bf2f(gc[n].s[g]);
-        U4 b[GS];
+        const float s = bf2f(gc[n].s[g]), zs = s * (HASZ ? -16.f - (float)gc[n].z[g] : -24.f);
 #pragma unroll
-        for (int j = 0; j < GS; ++j) b[j] = dec8(ww[g * GS + j]);
-        f32x4_t d[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = HASZ ? xs[i] * (-16.f - (float)gc[n].z[g]) : xs[i];
-#pragma unroll
-        for (int j = 0; j < GS; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[i] = mfma32(xa[i][j], b[j], d[i]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i][n] += d[i] * s;
+        for (int i = 0; i < 4; ++i) {
+          acc[i][n] += d[i][n] * s;
+          acc[i][n] += xs[i] * zs;
+        }
       }
     }
   }
+  // each half of the waves finishes two of a wave's four output tiles
   q_wait_vm<0>();
+  __syncthreads();
+  float* red = (float*)smem + wn * 2048;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int n = 0; n < 4; ++n)
+    if ((n >> 1) != half) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+      for (int i = 0; i < 4; ++i)
+        *(f32x4_t*)(red + half * 8192 + ((n & 1) * 4 + i) * 256 + lane * 4) = acc[i][n];
+    }
+  __syncthreads();
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int m = m0 + wm * 64 + i * 16 + q * 4 + r, col = (nb + wn * 4 + n) * 16 + n16;
-        if (m < a.M && col < a.N) {
-          if (a.part) a.part[((long)sp * a.M + m) * a.N + col] = acc[i][n][r];
-          else int4_finish<GS>(a, m, col, acc[i][n][r]);
+  for (int n = 0; n < 4; ++n)
+    if ((n >> 1) == half) {
+      const int col = (nb + wn * 4 + n) * 16 + n16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4_t o = *(const f32x4_t*)(red + (1 - half) * 8192 + ((n & 1) * 4 + i) * 256 + lane * 4);
+        const f32x4_t v = half ? o + acc[i][n] : acc[i][n] + o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int m = m0 + i * 16 + q * 4 + r;
+          if (m < a.M && col < a.N) {
+            if (a.part) a.part[((long)sp * a.M + m) * a.N + col] = v[r];
+            else int4_finish<GS>(a, m, col, v[r]);
+          }
         }
       }
+    }
 }
 
 // y = act(sum of the splits + bias), V outputs of a row a thread
@@ -397,6 +412,9 @@ namespace {
 // Workgroups wanted: one a CU.  Two a CU measured 104.7 against 94.1 us on 256 x 2048 x 20480 and 18.4
 // against 14.2 us on 16 x 8192 x 8192 (more partial sums to write and join); 1 x 2048 x 20480 is the same.
 constexpr int Q_WGS = 256;
+#ifndef QLEAST
+#define QLEAST 4
+#endif
 struct Plan4 { int tile, mt, nt, mb, nb, splits; };
 Plan4 plan4(int M, int N, int K, bool aligned) {
   Plan4 p;
@@ -404,11 +422,9 @@ Plan4 plan4(int M, int N, int K, bool aligned) {
   p.tile = aligned && M > 32;
   long least;  // tiles of a split at least
   if (p.tile) {
-    p.mt = M <= 64 ? 1 : 2;
-    p.nt = 4;
-    p.mb = (M + 64 * p.mt - 1) / (64 * p.mt);
-    p.nb = (N + 64 * p.nt - 1) / (64 * p.nt);
-    least = 4;
+    p.mb = (M + QT_M - 1) / QT_M;
+    p.nb = (N + QT_N - 1) / QT_N;
+    least = QLEAST;
   } else {
     p.mt = M <= 16 ? 1 : 2;
     p.nt = M <= 8 ? 1 : 2;
@@ -429,21 +445,20 @@ void go4(const Plan4& p, const Args4& a, hipStream_t st) {
   if (a.z) int4_mm_k<MT, NT, NW, GS, true><<<grid, NW * 64, 0, st>>>(a);
   else int4_mm_k<MT, NT, NW, GS, false><<<grid, NW * 64, 0, st>>>(a);
 }
-template <int WM, int WN, int NS, int GS>
+template <int GS>
 void go4t(const Plan4& p, const Args4& a, hipStream_t st) {
-  auto kern = a.z ? int4_tile_k<WM, WN, NS, GS, true> : int4_tile_k<WM, WN, NS, GS, false>;
-  constexpr int lds = Tile4<WM, WN, NS>::LDS;
-  static bool set[2];  // per kernel; setting it twice is harmless
+  auto kern = a.z ? int4_tile_k<GS, true> : int4_tile_k<GS, false>;
+  constexpr int lds = QR * Q_STAGE;
+  static bool set[2];  // of these two kernels; setting it twice is harmless
   if (!set[a.z != nullptr]) {
     (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     set[a.z != nullptr] = true;
   }
-  kern<<<p.mb * p.nb * p.splits, WM * WN * 64, lds, st>>>(a, p.mb, p.nb, p.splits);
+  kern<<<p.mb * p.nb * p.splits, 512, lds, st>>>(a, p.mb, p.nb, p.splits);
 }
 template <int GS>
 int go4g(const Plan4& p, const Args4& a, hipStream_t st) {
-  if (p.tile && p.mt == 1) go4t<1, 4, 3, GS>(p, a, st);
-  else if (p.tile) go4t<2, 4, 3, GS>(p, a, st);
+  if (p.tile) go4t<GS>(p, a, st);
   else if (p.mt == 1 && p.nt == 1) go4<1, 1, 16, GS>(p, a, st);
   else if (p.mt == 1) go4<1, 2, 16, GS>(p, a, st);
   else go4<2, 2, 8, GS>(p, a, st);
