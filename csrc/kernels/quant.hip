@@ -264,8 +264,8 @@ __global__ __launch_bounds__(512) void int4_tile_k(Args4 a, int mb, int nbk, int
     wo[j] = ((uint32_t)(wid * 2 + j) * (uint32_t)kt + (uint32_t)t0) * 1024u + (uint32_t)lane * 16u;
   }
   // stages past the end are issued too, out of range (zeros, no traffic): the count of loads in flight stays known
-  auto issue = [&](int t, int slot) {
-    unsigned char* base = smem + slot * Q_STAGE + wid * 2048;
+  auto issue = [&](int t, unsigned char* base) {
+    base += wid * 2048;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (q_lds_t*)(base + j * 1024), 16,
@@ -304,23 +304,18 @@ __global__ __launch_bounds__(512) void int4_tile_k(Args4 a, int mb, int nbk, int
   asm volatile("" : "+v"(e16));  // in a vector register: and-or takes one scalar
   scales(half);
 #pragma unroll
-  for (int t = 0; t < QR - 2; ++t) issue(t, t);
-  int slot = 0, free = QR - 2;  // of stage t; of stage t + QR - 2
-  for (int t = 0; t < nk; t += 2) {
-    q_wait_vm<4 * (QR - 4)>();     // this wave's part of stages t and t + 1 has landed
-    __builtin_amdgcn_s_barrier();  // and every wave's; all have left the buffers of the two before
-    asm volatile("" ::: "memory");
+  for (int t = 0; t < QR - 2; ++t) issue(t, smem + t * Q_STAGE);
+  // One pair of stages.  `st` is what this wave works on, f0 and f1 where stages t + QR - 2 and t + QR - 1 go:
+  // as separate restricted arguments, or the compiler would drain the loads in flight before an LDS read.
+  auto pair = [&](int t, const unsigned char* __restrict__ st, unsigned char* __restrict__ f0,
+                  unsigned char* __restrict__ f1) __attribute__((always_inline)) {
     Group<GS> gc[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) gc[n] = gn[n];
     scales(t + 2 + half);
-    issue(t + QR - 2, free);
-    free = free + 1 == QR ? 0 : free + 1;
-    issue(t + QR - 1, free);
-    free = free + 1 == QR ? 0 : free + 1;
-    const int other = slot + 1 == QR ? 0 : slot + 1;
-    const unsigned char* st = smem + (half ? other : slot) * Q_STAGE;
-    slot = other + 1 == QR ? 0 : other + 1;
+    issue(t + QR - 2, f0);
+    issue(t + QR - 1, f1);
+    __builtin_amdgcn_sched_barrier(0);
     const unsigned char* sx = st + n16 * 256;
     U4 wv[4];
 #pragma unroll
@@ -355,37 +350,43 @@ __global__ __launch_bounds__(512) void int4_tile_k(Args4 a, int mb, int nbk, int
         }
       }
     }
+  };
+  int slot = 0, fill = QR - 2;  // of stage t; of stage t + QR - 2
+  for (int t = 0; t < nk; t += 2) {
+    q_wait_vm<4 * (QR - 4)>();     // this wave's part of stages t and t + 1 has landed
+    __builtin_amdgcn_s_barrier();  // and every wave's; all have left the buffers of the two before
+    asm volatile("" ::: "memory");
+    const int slot1 = slot + 1 == QR ? 0 : slot + 1, fill1 = fill + 1 == QR ? 0 : fill + 1;
+    pair(t, smem + (half ? slot1 : slot) * Q_STAGE, smem + fill * Q_STAGE, smem + fill1 * Q_STAGE);
+    slot = slot1 + 1 == QR ? 0 : slot1 + 1;
+    fill = fill1 + 1 == QR ? 0 : fill1 + 1;
   }
-  // each half of the waves finishes two of a wave's four output tiles
+  // The halves meet in LDS, [half][64 rows][256 + 4 outputs]; then all 512 threads write rows of 4 outputs.
   q_wait_vm<0>();
   __syncthreads();
-  float* red = (float*)smem + wn * 2048;
+  float* red = (float*)smem;
+  constexpr int RS = QT_N + 4, RH = QT_M * RS;
 #pragma unroll
-  for (int n = 0; n < 4; ++n)
-    if ((n >> 1) != half) {
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *(f32x4_t*)(red + half * 8192 + ((n & 1) * 4 + i) * 256 + lane * 4) = acc[i][n];
-    }
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        red[half * RH + (i * 16 + q * 4 + r) * RS + (wn * 4 + n) * 16 + n16] = acc[i][n][r];
   __syncthreads();
-#pragma unroll
-  for (int n = 0; n < 4; ++n)
-    if ((n >> 1) == half) {
-      const int col = (nb + wn * 4 + n) * 16 + n16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4_t o = *(const f32x4_t*)(red + (1 - half) * 8192 + ((n & 1) * 4 + i) * 256 + lane * 4);
-        const f32x4_t v = half ? o + acc[i][n] : acc[i][n] + o;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int m = m0 + i * 16 + q * 4 + r;
-          if (m < a.M && col < a.N) {
-            if (a.part) a.part[((long)sp * a.M + m) * a.N + col] = v[r];
-            else int4_finish<GS>(a, m, col, v[r]);
-          }
-        }
-      }
+  const int c = lane * 4, col = nb * 16 + c, cols = min(a.N - col, 4);
+#pragma unroll 1
+  for (int r = wid; r < min(a.M - m0, QT_M); r += 8) {
+    const f32x4_t v = *(const f32x4_t*)(red + r * RS + c) + *(const f32x4_t*)(red + RH + r * RS + c);
+    if (a.part) {
+      float* o = a.part + ((long)sp * a.M + m0 + r) * a.N + col;
+      if (cols == 4) __builtin_memcpy(o, &v, 16);
+      else
+        for (int k = 0; k < cols; ++k) o[k] = v[k];
+    } else {
+      for (int k = 0; k < cols; ++k) int4_finish<GS>(a, m0 + r, col + k, v[k]);
     }
+  }
 }
 
 // y = act(sum of the splits + bias), V outputs of a row a thread
