@@ -77,12 +77,13 @@ PTG_DEV void int4_finish(const Args4& a, int m, int n, float s) {
 
 }  // namespace
 
-// A wave computes 16 * MT rows x 16 * NT outputs over its share of K; the NW waves of a workgroup take the
-// tiles of the workgroup's K range in turn and are joined in LDS in a fixed order.  One wave is one MFMA
-// chain a product tile: sum (16 + u) x on top of -(16 + z) * sum x, the latter from one MFMA with ones for
-// every 32 inputs that all NT tiles share.  The next tile's weights, scales and inputs are loaded before
-// the current tile is worked on.  Where K is split
-// over workgroups they leave fp32 sums in part[split][M][N], else they finish y.
+// Up to 32 rows: bound by reading the weights once.  A wave computes 16 * MT rows x 16 * NT outputs over its
+// share of K; the NW waves of a workgroup take the tiles of the workgroup's K range in turn and are joined
+// in LDS in a fixed order.  A product tile is one MFMA chain: sum (16 + u) x on top of -(16 + z) * sum x,
+// the latter from one MFMA with ones for every 32 inputs that all NT tiles share.  Waves that need few
+// registers hide the memory's latency, not loads ahead of their use: with 2 or 3 tiles in flight a wave
+// (88 or 122 registers instead of 62) 1 x 2048 x 20480 took 11.1 or 11.3 us instead of 9.5.
+// Where K is split over workgroups they leave fp32 sums in part[split][M][N], else they finish y.
 template <int GS>
 struct Group {  // of a tile: 4 / GS groups
   static constexpr int NG = 4 / GS;
@@ -96,60 +97,39 @@ __global__ __launch_bounds__(NW * 64) void int4_mm_k(Args4 a) {
   __shared__ float red[(FLAT ? NW : NW / 2) * R][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, q = lane >> 4;
   const int sp = blockIdx.x, splits = gridDim.x, nb = blockIdx.y * NT, m0 = blockIdx.z * 16 * MT;
-  const int M = a.M, N = a.N, K = a.K, kt = a.kt;
-  const bf16_t* __restrict__ x = a.x;
-  const uint8_t* __restrict__ w = a.w;
-  const bf16_t* __restrict__ scale = a.s;
-  const uint8_t* __restrict__ zero = a.z;
-  const int ntiles = (N + 15) / 16;
+  const int M = a.M, N = a.N, K = a.K, kt = a.kt, ntiles = (N + 15) / 16;
   const int t0 = (int)((long)kt * sp / splits), t1 = (int)((long)kt * (sp + 1) / splits);
-  const bf16_t* xr[MT];
-  bool mon[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = m0 + i * 16 + n16;
-    mon[i] = m < M;
-    xr[i] = x + (long)(mon[i] ? m : 0) * K + q * 8;
-  }
+  // rows, tiles of outputs and inputs that do not exist read 0
+  const Rsrc rx = make_rsrc(a.x + (long)m0 * K, (uint32_t)min(M - m0, 16 * MT) * (uint32_t)K * 2u);
+  const Rsrc rw = make_rsrc(a.w + (long)nb * kt * 1024, (uint32_t)min(ntiles - nb, NT) * (uint32_t)kt * 1024u);
   f32x4_t acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[i][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  U4 wn[NT], xn[MT][4];
-  Group<GS> gn[NT];
-  auto fetch = [&](int t) {
+  struct Tile {
+    U4 w[NT], x[MT][4];
+    Group<GS> g[NT];
+  };
+  auto fetch = [&](Tile& f, int t) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int nt = nb + n < ntiles ? nb + n : ntiles - 1;  // a tile that is not there: any, not stored
-      const long tile = (long)nt * kt + t;
-      wn[n] = *(const U4*)(w + tile * 1024 + lane * 16);
-      __builtin_memcpy(gn[n].s, scale + (tile * 16 + n16) * NG, 2 * NG);
-      if (HASZ) __builtin_memcpy(gn[n].z, zero + (tile * 16 + n16) * NG, NG);
+      f.w[n] = bload16(rw, ((uint32_t)n * (uint32_t)kt + (uint32_t)t) * 1024u + lane * 16u);
+      const long at = (((long)min(nb + n, ntiles - 1) * kt + t) * 16 + n16) * NG;
+      __builtin_memcpy(f.g[n].s, a.s + at, 2 * NG);
+      if (HASZ) __builtin_memcpy(f.g[n].z, a.z + at, NG);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        xn[i][j] = zero4();
-        if (mon[i] && t * QT_K + j * 32 + q * 8 < K) __builtin_memcpy(&xn[i][j], xr[i] + t * QT_K + j * 32, 16);
+        const int k = t * QT_K + j * 32 + q * 8;
+        f.x[i][j] = bload16(rx, k < K ? ((uint32_t)(i * 16 + n16) * (uint32_t)K + (uint32_t)k) * 2u : PTG_OOB);
       }
   };
   U4 ones;
   ones.x = 0x3F803F80u; ones.y = ones.x; ones.z = ones.x; ones.w = ones.x;
-  int t = t0 + wave;
-  if (t < t1) fetch(t);
-  while (t < t1) {
-    U4 wc[NT], xc[MT][4];
-    Group<GS> gc[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) { wc[n] = wn[n]; gc[n] = gn[n]; }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) xc[i][j] = xn[i][j];
-    t += NW;
-    if (t < t1) fetch(t);
+  auto multiply = [&](const Tile& f) {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       f32x4_t xs[MT];  // sum of the group's inputs, the same in every column
@@ -157,13 +137,13 @@ __global__ __launch_bounds__(NW * 64) void int4_mm_k(Args4 a) {
       for (int i = 0; i < MT; ++i) {
         xs[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < GS; ++j) xs[i] = mfma32(xc[i][g * GS + j], ones, xs[i]);
+        for (int j = 0; j < GS; ++j) xs[i] = mfma32(f.x[i][g * GS + j], ones, xs[i]);
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const uint32_t ww[4] = {wc[n].x, wc[n].y, wc[n].z, wc[n].w};
-        const float s = bf2f(gc[n].s[g]);
-        const float zf = HASZ ? -16.f - (float)gc[n].z[g] : -24.f;
+        const uint32_t ww[4] = {f.w[n].x, f.w[n].y, f.w[n].z, f.w[n].w};
+        const float s = bf2f(f.g[n].s[g]);
+        const float zf = HASZ ? -16.f - (float)f.g[n].z[g] : -24.f;
         U4 b[GS];
 #pragma unroll
         for (int j = 0; j < GS; ++j) b[j] = dec8(ww[g * GS + j]);
@@ -171,11 +151,16 @@ __global__ __launch_bounds__(NW * 64) void int4_mm_k(Args4 a) {
         for (int i = 0; i < MT; ++i) {
           f32x4_t d = xs[i] * zf;
 #pragma unroll
-          for (int j = 0; j < GS; ++j) d = mfma32(xc[i][g * GS + j], b[j], d);
+          for (int j = 0; j < GS; ++j) d = mfma32(f.x[i][g * GS + j], b[j], d);
           acc[i][n] += d * s;
         }
       }
     }
+  };
+  for (int t = t0 + wave; t < t1; t += NW) {
+    Tile f;
+    fetch(f, t);
+    multiply(f);
   }
   auto put = [&](int slot) {
 #pragma unroll
@@ -410,32 +395,33 @@ __global__ __launch_bounds__(256) void int4_join_k(Args4 a, int splits) {
 }
 
 namespace {
-// Workgroups wanted: one a CU.  Two a CU measured 104.7 against 94.1 us on 256 x 2048 x 20480 and 18.4
-// against 14.2 us on 16 x 8192 x 8192 (more partial sums to write and join); 1 x 2048 x 20480 is the same.
-constexpr int Q_WGS = 256;
-#ifndef QLEAST
-#define QLEAST 4
-#endif
+constexpr int Q_NW = 16;  // waves of int4_mm_k
+// Above 32 rows the tile kernel: 32 x 8192 x 8192 measured 19.3 us with it and 22.9 without, but 32 x 2048 x
+// 20480 20.6 and 17.8, 12 x 8192 x 8192 17.3 and 12.1.
+//
+// Outputs alone give one workgroup a CU only where N is large; otherwise K is split, up to one workgroup a
+// CU (two: 16 x 8192 x 8192 17.0 instead of 13.4 us, 12 x 2048 x 20480 13.9 instead of 10.9).  A split costs
+// the join, about 2.2 us, so a wave keeps at least 4 tiles (one row: 4 x 2048 x 8192 7.2 us whole, 9.4 in two)
+// or 2 where it works on two columns of tiles at a time (12 x 2048 x 20480 10.9 us in four, 22.5 whole).
 struct Plan4 { int tile, mt, nt, mb, nb, splits; };
-Plan4 plan4(int M, int N, int K, bool aligned) {
+Plan4 plan4(int M, int N, int K) {
   Plan4 p;
   const long kt = (K + QT_K - 1) / QT_K;
-  p.tile = aligned && M > 32;
+  p.tile = M > 32;
   long least;  // tiles of a split at least
   if (p.tile) {
     p.mb = (M + QT_M - 1) / QT_M;
     p.nb = (N + QT_N - 1) / QT_N;
-    least = QLEAST;
+    least = 4;
   } else {
     p.mt = M <= 16 ? 1 : 2;
-    p.nt = M <= 8 ? 1 : 2;
+    p.nt = M <= 8 ? 1 : 2;  // two: half the reads of the inputs; 16 x 8192 x 8192 13.4 us instead of 19.5
     p.mb = (M + 16 * p.mt - 1) / (16 * p.mt);
     p.nb = (N + 16 * p.nt - 1) / (16 * p.nt);
-    least = 2 * (p.mt == 1 ? 16 : 8);  // two a wave
+    least = Q_NW * (p.nt == 1 ? 4 : 2);
   }
   const long wgs = (long)p.nb * p.mb;
-  long s = (Q_WGS + wgs - 1) / wgs;
-  if (p.tile) s = Q_WGS / wgs;
+  long s = p.tile ? 256 / wgs : (256 + wgs - 1) / wgs;
   if (s > kt / least) s = kt / least;
   p.splits = s < 1 ? 1 : (int)s;
   return p;
@@ -460,9 +446,9 @@ void go4t(const Plan4& p, const Args4& a, hipStream_t st) {
 template <int GS>
 int go4g(const Plan4& p, const Args4& a, hipStream_t st) {
   if (p.tile) go4t<GS>(p, a, st);
-  else if (p.mt == 1 && p.nt == 1) go4<1, 1, 16, GS>(p, a, st);
-  else if (p.mt == 1) go4<1, 2, 16, GS>(p, a, st);
-  else go4<2, 2, 8, GS>(p, a, st);
+  else if (p.mt == 1 && p.nt == 1) go4<1, 1, Q_NW, GS>(p, a, st);
+  else if (p.mt == 1) go4<1, 2, Q_NW, GS>(p, a, st);
+  else go4<2, 2, Q_NW, GS>(p, a, st);
   if (a.part) {
     const long total = (long)a.M * a.N;
     if (a.N % 4 == 0) int4_join_k<GS, 4><<<(int)((total / 4 + 255) / 256), 256, 0, st>>>(a, p.splits);
@@ -476,23 +462,19 @@ extern "C" {
 
 // *floats: workspace of a product of M rows (0 where none is needed)
 int ptg_int4_ws(int M, int N, int K, void* floats) {
-  long most = 0;
-  for (int al = 0; al < 2 && M > 0; ++al) {
-    const Plan4 p = plan4(M, N, K, al != 0);
-    if (p.splits > 1 && p.splits > most) most = p.splits;
-  }
-  *(long*)floats = most * M * N;
+  const int splits = M > 0 ? plan4(M, N, K).splits : 1;
+  *(long*)floats = splits > 1 ? (long)splits * M * N : 0;
   return 0;
 }
 
-// w, scale, zero: tile layout; group 32, 64 or 128; zero null: 8 everywhere; act 0 linear, 1 ReLU
+// x: 16-byte aligned; w, scale, zero: tile layout; group 32, 64 or 128; zero null: 8 everywhere; act 0 linear, 1 ReLU
 int ptg_int4_dense(const void* x, const void* w, const void* scale, const void* zero, const void* bias, void* y,
                    void* ws, int M, int N, int K, int group, int act, int f32, hipStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   // a block of rows or of outputs stays below 2 GiB
-  if ((group != 32 && group != 64 && group != 128) || K < group || K % group || K > (1 << 22))
+  if ((group != 32 && group != 64 && group != 128) || K < group || K % group || K > (1 << 22) || ((uintptr_t)x & 15))
     return (int)hipErrorInvalidValue;
-  const Plan4 p = plan4(M, N, K, ((uintptr_t)x & 15) == 0);
+  const Plan4 p = plan4(M, N, K);
   if (p.splits > 1 && !ws) return (int)hipErrorInvalidValue;
   const Args4 a{(const bf16_t*)x, (const uint8_t*)w, (const bf16_t*)scale, (const uint8_t*)zero, (const float*)bias,
                 y, p.splits > 1 ? (float*)ws : nullptr, M, N, K, (K + QT_K - 1) / QT_K, act, f32};

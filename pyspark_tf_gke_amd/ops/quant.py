@@ -190,6 +190,8 @@ def int4_dense_fwd(x, w: Int4Weight, bias, act, out, workspace=None):
         return out
     if x.dtype != torch.bfloat16:
         raise TypeError(f"int4_dense: x must be bfloat16, got {x.dtype}")
+    if x.data_ptr() & 15:
+        x = x.clone()  # the kernel reads 16 bytes at a time
     need = int4_workspace_floats(B, w)
     if need and workspace is None:
         workspace = torch.empty(need, dtype=torch.float32, device=dev)
