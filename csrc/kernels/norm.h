@@ -222,6 +222,7 @@ struct Lane {
 struct ColVec {
   const float* src;  // null: dflt everywhere
   float dflt;
+  float mul;  // times this
 };
 template <int NT, int N>
 struct ColVecs {
@@ -248,6 +249,10 @@ struct ColVecs {
         }
       }
 #pragma unroll
+      for (int k = 0; k < N; ++k) {
+        t[k].x *= v[k].mul; t[k].y *= v[k].mul; t[k].z *= v[k].mul; t[k].w *= v[k].mul;
+      }
+#pragma unroll
       for (int k = 0; k < N; ++k) *(float4*)(lds + 2 * k * half + ((c >> 2) & 1) * half + (c >> 3) * 4) = t[k];
     }
   }
@@ -258,11 +263,15 @@ struct ColVecs {
       const float4 a = *(const float4*)p, b = *(const float4*)(p + half);
       f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
       f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else if (v[k].src && nv == 8) {
-      __builtin_memcpy(f, v[k].src + c0, 32);
     } else {
+      if (v[k].src && nv == 8) {
+        __builtin_memcpy(f, v[k].src + c0, 32);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = v[k].src && j < nv ? v[k].src[c0 + j] : v[k].dflt;
+        for (int j = 0; j < 8; ++j) f[j] = v[k].src && j < nv ? v[k].src[c0 + j] : v[k].dflt;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= v[k].mul;
     }
   }
 };

@@ -10,34 +10,31 @@
 // workgroups' partial sums in a fixed order: no atomics, the same bits every run.  As in the forward pass
 // the next row's loads are in flight while a row is worked on.
 #include "norm.h"
-#ifndef BWD_OCC
-#define BWD_OCC 2
-#endif
 
-// Joins a thread's column sums over the rows (slots) of the workgroup and writes dst[0..C).
-template <int LPR, int NT, typename D>
-PTG_DEV void flush_cols(float* acc, float* lds, int tid, int tpr, int C, D* dst) {
-  constexpr int NW = NT / 64;
-  int rows, cols;
+// A thread's column sums over the rows (slots) of the workgroup: put_cols leaves them in LDS, [rows][cols]
+// (col_floats in all), and sum_cols adds dst[0..C) up after a barrier.
+template <int LPR, int NT>
+PTG_DEV int col_rows(int tpr) { return LPR < 64 ? NT / 64 : NT / tpr; }
+template <int LPR, int NT>
+constexpr int col_floats() { return LPR < 64 ? NT / 64 * LPR * 8 : NT * 8; }
+template <int LPR, int NT>
+PTG_DEV void put_cols(float* acc, float* lds, int tid, float mul) {
   if (LPR < 64) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
 #pragma unroll
       for (int o = LPR; o < 64; o <<= 1) acc[j] += __shfl_xor(acc[j], o, 64);
     }
-    rows = NW;
-    cols = LPR * 8;
-  } else {
-    rows = NT / tpr;
-    cols = tpr * 8;
   }
-  __syncthreads();
   if (LPR == 64 || (tid & 63) < LPR) {
-    const int r = LPR < 64 ? tid >> 6 : tid / tpr, c = LPR < 64 ? (tid & 63) * 8 : (tid % tpr) * 8;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) lds[r * cols + c + j] = acc[j];
+    float* p = lds + (LPR < 64 ? (tid >> 6) * LPR * 8 + (tid & 63) * 8 : tid * 8);
+    *(float4*)p = make_float4(acc[0] * mul, acc[1] * mul, acc[2] * mul, acc[3] * mul);
+    *(float4*)(p + 4) = make_float4(acc[4] * mul, acc[5] * mul, acc[6] * mul, acc[7] * mul);
   }
-  __syncthreads();
+}
+template <int LPR, int NT, typename D>
+PTG_DEV void sum_cols(const float* lds, int tid, int tpr, int C, D* dst) {
+  const int rows = col_rows<LPR, NT>(tpr), cols = LPR < 64 ? LPR * 8 : tpr * 8;
   for (int c = tid; c < C; c += NT) {
     float s = 0.f;
     for (int r = 0; r < rows; ++r) s += lds[r * cols + c];
@@ -45,6 +42,9 @@ PTG_DEV void flush_cols(float* acc, float* lds, int tid, int tpr, int C, D* dst)
     else dst[c] = s;
   }
 }
+// vectors joined at a time at the end: what LDS holds next to the column vectors
+template <int NT>
+constexpr int flush_vecs() { return NT <= 512 ? 5 : 3; }
 
 template <typename T>
 struct RowIn {  // a row on its way in
@@ -73,7 +73,7 @@ PTG_DEV void load_row(RowIn<T>& in, const BlkArgs& a, const Lane<T, ALN>& ln, lo
 }
 
 template <typename T, int LPR, int NT, bool ALN, bool PO, bool PR, bool GG, bool DROP>
-__global__ __launch_bounds__(NT, BWD_OCC) void block_norm_bwd_k(BlkArgs a) {
+__global__ __launch_bounds__(NT, 2) void block_norm_bwd_k(BlkArgs a) {
   __shared__ float2 xch[2 * (NT / 64)];
   extern __shared__ float4 dyn[];
   float* vecs = (float*)dyn;  // column vectors, then [NT * 8] of the joins
@@ -93,16 +93,16 @@ __global__ __launch_bounds__(NT, BWD_OCC) void block_norm_bwd_k(BlkArgs a) {
   load_row<ALN, PO, PR>(in, a, ln, it.base, rows, on);
   ColVecs<NT, 4> cv;
   enum { G1, B1, G2, GV };
-  cv.v[G1] = {PO ? a.g1 : nullptr, 1.f};
-  cv.v[B1] = {PO ? a.b1 : nullptr, 0.f};
-  cv.v[G2] = {PR ? a.g2 : nullptr, 1.f};
-  cv.v[GV] = {a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, 1.f};
+  cv.v[G1] = {PO ? a.g1 : nullptr, 1.f, 1.f};
+  cv.v[B1] = {PO ? a.b1 : nullptr, 0.f, 1.f};
+  cv.v[G2] = {PR ? a.g2 : nullptr, 1.f, 1.f};
+  const float fs = DROP ? a.scale * a.d.scale : a.scale;  // scale and keep scale, times the gate: gt
+  cv.v[GV] = {a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, 1.f, fs};
   cv.init(vecs, C, tid);
   float* cols = vecs + (cv.LDS ? 8 * cv.half : 0);
   float ag1[8], ab1[8], ag2[8], ab2[8], agt[8], gt[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) { ag1[j] = 0.f; ab1[j] = 0.f; ag2[j] = 0.f; ab2[j] = 0.f; agt[j] = 0.f; gt[j] = 1.f; }
-  const float fs = DROP ? a.scale * a.d.scale : a.scale;  // of a kept element
+  for (int j = 0; j < 8; ++j) { ag1[j] = 0.f; ab1[j] = 0.f; ag2[j] = 0.f; ab2[j] = 0.f; agt[j] = 0.f; gt[j] = fs; }
   // the sums' shares: mean(g) of a LayerNorm only, mean(g * xhat) of a norm only
   const float p1 = a.kind1 == NORM_LAYER ? rx.invC : 0.f, q1 = a.kind1 ? rx.invC : 0.f;
   const float p2 = a.kind2 == NORM_LAYER ? rx.invC : 0.f;
@@ -129,6 +129,8 @@ __global__ __launch_bounds__(NT, BWD_OCC) void block_norm_bwd_k(BlkArgs a) {
     if (GG && first) {
       gl.load(t, a.gate, (g + (a.slotwise ? slot : 0)) * C, 0, C, con);
       t.get(gt);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gt[j] *= fs;
     }
     if (PO) {
       float b[8];
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(NT, BWD_OCC) void block_norm_bwd_k(BlkArgs a) {
       cv.get(vecs, G2, v, cc, nv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float k = n[j] * gt[j] * fs;
+        const float k = n[j] * gt[j];
         r[j] = (r[j] + (!DROP || keep[j] ? k : 0.f) - m2) * s2;  // xhat of h
         if (!ALN) r[j] = j < nv ? r[j] : 0.f;
         ag2[j] = fmaf(gu[j], r[j], ag2[j]);
@@ -169,7 +171,7 @@ __global__ __launch_bounds__(NT, BWD_OCC) void block_norm_bwd_k(BlkArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float dd = !DROP || keep[j] ? gh[j] * fs : 0.f;
+      const float dd = !DROP || keep[j] ? gh[j] : 0.f;  // times fs: in gt, and in agt where it is flushed
       agt[j] = fmaf(dd, n[j], agt[j]);
       gh[j] = dd * gt[j];
     }
@@ -196,12 +198,16 @@ __global__ __launch_bounds__(NT, BWD_OCC) void block_norm_bwd_k(BlkArgs a) {
     }
     if (GG && last) {
       if (a.slotwise) {  // this slot has its whole group: the sums are final
+#pragma unroll
+        for (int j = 0; j < 8; ++j) agt[j] *= fs;
         t.set(agt);
         gl.store(t, a.dgate, (g + slot) * C, 0, C, con);
-      } else if (a.sub > 1) {
-        flush_cols<LPR, NT>(agt, cols, tid, tpr, C, a.gpart + item * C);
       } else {
-        flush_cols<LPR, NT>(agt, cols, tid, tpr, C, (T*)a.dgate + item * C);
+        __syncthreads();
+        put_cols<LPR, NT>(agt, cols, tid, fs);
+        __syncthreads();
+        if (a.sub > 1) sum_cols<LPR, NT>(cols, tid, tpr, C, a.gpart + item * C);
+        else sum_cols<LPR, NT>(cols, tid, tpr, C, (T*)a.dgate + item * C);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) agt[j] = 0.f;
@@ -209,63 +215,82 @@ __global__ __launch_bounds__(NT, BWD_OCC) void block_norm_bwd_k(BlkArgs a) {
   }
   // partial column sums: [vector][workgroup][C], vectors in the order dgamma2, dbeta2, dgamma1,
   // dbeta1, dgate as far as they are there (nvec)
-  const long wg = (long)gridDim.x * C;
   float* p = a.part + (long)blockIdx.x * C;
+  int v = 0;
+  auto drain = [&] {
+    __syncthreads();
+    for (int k = 0; k < v; ++k, p += (long)gridDim.x * C) sum_cols<LPR, NT>(cols + k * col_floats<LPR, NT>(), tid, tpr, C, p);
+    v = 0;
+  };
+  auto flush = [&](float* acc, float mul) {
+    if (v == flush_vecs<NT>()) {
+      drain();
+      __syncthreads();
+    }
+    put_cols<LPR, NT>(acc, cols + v++ * col_floats<LPR, NT>(), tid, mul);
+  };
+  __syncthreads();
   if (PR) {
-    flush_cols<LPR, NT>(ag2, cols, tid, tpr, C, p);
-    p += wg;
-    if (a.kind2 == NORM_LAYER) { flush_cols<LPR, NT>(ab2, cols, tid, tpr, C, p); p += wg; }
+    flush(ag2, 1.f);
+    if (a.kind2 == NORM_LAYER) flush(ab2, 1.f);
   }
   if (PO && a.kind1) {
-    flush_cols<LPR, NT>(ag1, cols, tid, tpr, C, p);
-    p += wg;
-    if (a.kind1 == NORM_LAYER) { flush_cols<LPR, NT>(ab1, cols, tid, tpr, C, p); p += wg; }
+    flush(ag1, 1.f);
+    if (a.kind1 == NORM_LAYER) flush(ab1, 1.f);
   }
-  if (a.gate_mode == GATE_VEC) flush_cols<LPR, NT>(agt, cols, tid, tpr, C, p);
+  if (a.gate_mode == GATE_VEC) flush(agt, fs);
+  drain();
 }
 
-// Sums of up to 5 [rows][C] matrices over their rows, in a fixed order: 32 columns and 32 strips of
-// rows a workgroup.  A gradient that is not asked for has a null destination.
+// The sums of the workgroups' parts, in a fixed order.  First `cblocks` workgroups a vector: sums of up to
+// 5 [rows][C] matrices over their rows, 32 columns and 32 strips of rows a workgroup (a gradient that is
+// not asked for has a null destination).  Then dgate[g][c] = sum of the `sub` partial rows of group g.
 struct ColSums {
   const float* src;
   float* dst[5];
+  const float* gsrc;
+  void* gdst;
+  long gn;
+  int rows, C, cblocks, nvec, sub;
 };
-__global__ __launch_bounds__(1024) void col_sums_k(ColSums a, int rows, int C) {
+template <typename T>
+__global__ __launch_bounds__(1024) void col_sums_k(ColSums a) {
   __shared__ float s[32][33];
-  if (!a.dst[blockIdx.y]) return;
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
-  const float* p = a.src + (long)blockIdx.y * rows * C;
+  const int C = a.C;
+  if ((int)blockIdx.x >= a.cblocks * a.nvec) {
+    const long i = (long)(blockIdx.x - a.cblocks * a.nvec) * 1024 + threadIdx.x;
+    if (i >= a.gn) return;
+    const long g = i / C;
+    const float* p = a.gsrc + g * a.sub * C + (i - g * C);
+    float v = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < a.sub; ++k) v += p[(long)k * C];
+    if constexpr (sizeof(T) == 2) ((T*)a.gdst)[i] = f2bf(v);
+    else ((T*)a.gdst)[i] = v;
+    return;
+  }
+  const int y = blockIdx.x / a.cblocks;
+  if (!a.dst[y]) return;
+  const int c = (blockIdx.x - y * a.cblocks) * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+  const float* p = a.src + (long)y * a.rows * C;
   float v = 0.f;
-  if (c < C)
-    for (int r = k; r < rows; r += 32) v += p[(long)r * C + c];
+  if (c < C) {
+#pragma unroll 8
+    for (int r = k; r < a.rows; r += 32) v += p[(long)r * C + c];
+  }
   s[k][threadIdx.x & 31] = v;
   __syncthreads();
   if (k == 0 && c < C) {
     v = 0.f;
 #pragma unroll
     for (int r = 0; r < 32; ++r) v += s[r][threadIdx.x];
-    a.dst[blockIdx.y][c] = v;
+    a.dst[y][c] = v;
   }
-}
-// dgate[g][c] = sum of the `sub` partial rows of group g
-template <typename T>
-__global__ __launch_bounds__(256) void gate_sums_k(const float* src, T* dst, long n, int C, int sub) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const long g = i / C;
-  const float* p = src + g * sub * C + (i - g * C);
-  float v = 0.f;
-  for (int k = 0; k < sub; ++k) v += p[(long)k * C];
-  if constexpr (sizeof(T) == 2) dst[i] = f2bf(v);
-  else dst[i] = v;
 }
 
 namespace {
 
-#ifndef BWD_WGS_
-#define BWD_WGS_ 256
-#endif
-constexpr int BWD_WGS = BWD_WGS_;  // workgroups of a backward pass at most: rows of its partial sums
+constexpr int BWD_WGS = 256;  // workgroups of a backward pass at most: rows of its partial sums
 
 struct Shape { int lpr, nt, tpr; };
 Shape shape_of(int C) {
@@ -294,14 +319,24 @@ void plan(BlkArgs& a, const Shape& s, int& grid) {
   grid = (int)(a.items < BWD_WGS ? a.items : BWD_WGS);
 }
 
+template <typename T, int LPR, int NT, bool ALN, bool PO, bool PR, bool GG, bool DROP>
+void bwd_run(const BlkArgs& a, int grid, hipStream_t st) {
+  auto kern = block_norm_bwd_k<T, LPR, NT, ALN, PO, PR, GG, DROP>;
+  const int lds = col_vec_bytes(NT, a.C, 4) + flush_vecs<NT>() * col_floats<LPR, NT>() * 4;
+  static bool set = false;  // setting it twice is harmless
+  if (LPR == 64 && !set) {
+    (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+    set = true;
+  }
+  kern<<<grid, NT, lds, st>>>(a);
+}
 template <typename T, bool ALN, bool PO, bool PR, bool GG, bool DROP>
 void bwd_go(const BlkArgs& a, const Shape& s, int grid, hipStream_t st) {
-  const int lds = col_vec_bytes(s.nt, a.C, 4) + s.nt * 8 * 4;
-  if (s.lpr == 2) block_norm_bwd_k<T, 2, 512, ALN, PO, PR, GG, DROP><<<grid, 512, lds, st>>>(a);
-  else if (s.lpr == 8) block_norm_bwd_k<T, 8, 512, ALN, PO, PR, GG, DROP><<<grid, 512, lds, st>>>(a);
-  else if (s.lpr == 32) block_norm_bwd_k<T, 32, 512, ALN, PO, PR, GG, DROP><<<grid, 512, lds, st>>>(a);
-  else if (s.nt == 512) block_norm_bwd_k<T, 64, 512, ALN, PO, PR, GG, DROP><<<grid, 512, lds, st>>>(a);
-  else block_norm_bwd_k<T, 64, 1024, ALN, PO, PR, GG, DROP><<<grid, 1024, lds, st>>>(a);
+  if (s.lpr == 2) bwd_run<T, 2, 512, ALN, PO, PR, GG, DROP>(a, grid, st);
+  else if (s.lpr == 8) bwd_run<T, 8, 512, ALN, PO, PR, GG, DROP>(a, grid, st);
+  else if (s.lpr == 32) bwd_run<T, 32, 512, ALN, PO, PR, GG, DROP>(a, grid, st);
+  else if (s.nt == 512) bwd_run<T, 64, 512, ALN, PO, PR, GG, DROP>(a, grid, st);
+  else bwd_run<T, 64, 1024, ALN, PO, PR, GG, DROP>(a, grid, st);
 }
 // no norm at all: the post-norm kernel, whose kind1 == 0 is the identity
 template <typename T, bool ALN, bool GG, bool DROP>
@@ -377,12 +412,14 @@ int ptg_block_norm_bwd(const void* x, const void* res, const void* gate, const v
   cs.src = a.part;
   if (f32) { if (aligned) bwd_mode<float, true>(a, s, grid, stream); else bwd_mode<float, false>(a, s, grid, stream); }
   else { if (aligned) bwd_mode<bf16_t, true>(a, s, grid, stream); else bwd_mode<bf16_t, false>(a, s, grid, stream); }
-  if (a.nvec) col_sums_k<<<dim3((C + 31) / 32, a.nvec), 1024, 0, stream>>>(cs, grid, C);
+  cs.rows = grid; cs.C = C; cs.nvec = a.nvec; cs.cblocks = (C + 31) / 32;
   if (gate_mode == GATE_GROUP && a.sub > 1) {
-    const long n = (M / rpg) * C;
-    const int blocks = (int)((n + 255) / 256);
-    if (f32) gate_sums_k<float><<<blocks, 256, 0, stream>>>(a.gpart, (float*)dgate, n, C, a.sub);
-    else gate_sums_k<bf16_t><<<blocks, 256, 0, stream>>>(a.gpart, (bf16_t*)dgate, n, C, a.sub);
+    cs.gsrc = a.gpart; cs.gdst = dgate; cs.gn = (M / rpg) * C; cs.sub = a.sub;
+  }
+  const long blocks = (long)cs.cblocks * cs.nvec + (cs.gn + 1023) / 1024;
+  if (blocks) {
+    if (f32) col_sums_k<float><<<(int)blocks, 1024, 0, stream>>>(cs);
+    else col_sums_k<bf16_t><<<(int)blocks, 1024, 0, stream>>>(cs);
   }
   PTG_RETURN_LAUNCH();
 }

@@ -29,13 +29,13 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
   Raw8<T> nx, nr, t;
   ln.load(nx, a.x, r0 * C, rows, C, on);
   ln.load(nr, a.res, r0 * C, rows, C, on);
-  cv.v[G1] = {PO ? a.g1 : nullptr, 1.f};
-  cv.v[B1] = {PO ? a.b1 : nullptr, 0.f};
-  cv.v[G2] = {PR ? a.g2 : nullptr, 1.f};
-  cv.v[B2] = {PR ? a.b2 : nullptr, 0.f};
-  cv.v[GV] = {a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, 1.f};
+  cv.v[G1] = {PO ? a.g1 : nullptr, 1.f, 1.f};
+  cv.v[B1] = {PO ? a.b1 : nullptr, 0.f, 1.f};
+  cv.v[G2] = {PR ? a.g2 : nullptr, 1.f, 1.f};
+  cv.v[B2] = {PR ? a.b2 : nullptr, 0.f, 1.f};
+  const float sc = DROP ? a.scale * a.d.scale : a.scale;  // scale and keep scale, times the gate
+  cv.v[GV] = {a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, 1.f, sc};
   cv.init(vecs, C, tid);
-  const float sc = DROP ? a.scale * a.d.scale : a.scale;
   const float lay1 = a.kind1 == NORM_LAYER ? 1.f : 0.f, lay2 = a.kind2 == NORM_LAYER ? 1.f : 0.f;
   const bool full = C == tpr * 8;
   __syncthreads();
@@ -60,26 +60,28 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = fmaf((f[j] - m1) * s1, v[j], w[j]);
     }
-    if (a.gate_mode) {
-      if (a.gate_mode == GATE_VEC) {
-        cv.get(vecs, GV, v, cc, nv);
-      } else if (con) {
+    if (a.gate_mode == GATE_GROUP) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      if (con) {
         const Lane<T, false> gl(0, c0, C);
         gl.load(t, a.gate, (cur + slot) / a.rpg * C, 0, C, true);
         t.get(v);
-      }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= v[j];
+        for (int j = 0; j < 8; ++j) v[j] *= sc;
+      }
+    } else {
+      cv.get(vecs, GV, v, cc, nv);
     }
     if (DROP) {
       bool keep[8];
       row_keep<ALN>(a, step, at, ln.off, keep);
       // a dropped value is 0 whatever the branch holds
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = r[j] + (keep[j] ? f[j] * sc : 0.f);
+      for (int j = 0; j < 8; ++j) f[j] = r[j] + (keep[j] ? f[j] * v[j] : 0.f);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = fmaf(f[j], sc, r[j]);
+      for (int j = 0; j < 8; ++j) f[j] = fmaf(f[j], v[j], r[j]);
     }
     if (!ALN || !full) {
 #pragma unroll
