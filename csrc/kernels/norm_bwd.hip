@@ -51,8 +51,8 @@ struct RowIn {  // a row on its way in
   Raw8<T> x, r, gu, gh;
   float m1, s1, m2, s2;
 };
-template <bool ALN, bool PO, bool PR, typename T>
-PTG_DEV void load_row(RowIn<T>& in, const BlkArgs& a, const Lane<T, ALN>& ln, long base, uint32_t rows, bool on) {
+template <bool PO, bool PR, typename T, typename L>
+PTG_DEV void load_row(RowIn<T>& in, const BlkArgs& a, const L& ln, long base, uint32_t rows, bool on) {
   const long at = base * a.C;
   ln.load(in.x, a.x, at, rows, a.C, on);
   if (PR) ln.load(in.r, a.res, at, rows, a.C, on);
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(NT, 2) void block_norm_bwd_k(BlkArgs a) {
   float* vecs = (float*)dyn;  // column vectors, then [NT * 8] of the joins
   const int tid = threadIdx.x, tpr = LPR < 64 ? LPR : a.tpr, slots = NT / tpr, slot = tid / tpr;
   const int C = a.C, c0 = (tid % tpr) * 8, lag = RowIter<GG>::lag(a, slot);
-  const Lane<T, ALN> ln(lag, c0, C);
+  const Lane<T, ALN, LPR == 2> ln(lag, c0, C);
   const int nv = ln.nv, cc = nv ? c0 : 0;
   RowX rx;
   rx.init(xch, tid, NT, LPR, tpr, C);
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(NT, 2) void block_norm_bwd_k(BlkArgs a) {
   it.enter(a, slots);
   uint32_t rows = it.rows(a, slots);
   bool on = lag < (int)rows && nv > 0;
-  load_row<ALN, PO, PR>(in, a, ln, it.base, rows, on);
+  load_row<PO, PR>(in, a, ln, it.base, rows, on);
   ColVecs<NT, 4> cv;
   enum { G1, B1, G2, GV };
   cv.v[G1] = {PO ? a.g1 : nullptr, 1.f, 1.f};
@@ -114,21 +114,21 @@ __global__ __launch_bounds__(NT, 2) void block_norm_bwd_k(BlkArgs a) {
     const bool con = on, first = it.j == 0, last = it.j == it.jn - 1;
     float xh[8], r[8], gu[8], gh[8], n[8], v[8];
     bool keep[8];
-    in.x.get(xh);
-    if (PR) in.r.get(r);
-    if (PR) in.gu.get(gu);
-    in.gh.get(gh);
+    ln.get(in.x, xh, on);
+    if (PR) ln.get(in.r, r, on);
+    if (PR) ln.get(in.gu, gu, on);
+    ln.get(in.gh, gh, on);
     const float m1 = in.m1, s1 = in.s1, m2 = in.m2, s2 = in.s2;
     it.next(a, slots);
     rows = it.item < a.items ? it.rows(a, slots) : 0;
     on = lag < (int)rows && nv > 0;
-    load_row<ALN, PO, PR>(in, a, ln, it.base, rows, on);
+    load_row<PO, PR>(in, a, ln, it.base, rows, on);
     if (DROP) row_keep<ALN>(a, step, at, ln.off, keep);
     Raw8<T> t;
-    const Lane<T, false> gl(0, c0, C);
+    const Lane<T, false, LPR == 2> gl(0, c0, C);
     if (GG && first) {
       gl.load(t, a.gate, (g + (a.slotwise ? slot : 0)) * C, 0, C, con);
-      t.get(gt);
+      gl.get(t, gt, con);
 #pragma unroll
       for (int j = 0; j < 8; ++j) gt[j] *= fs;
     }
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(NT, 2) void block_norm_bwd_k(BlkArgs a) {
       const float2 c = row_sum2<LPR>(make_float2(c1, c2), rx);
       const float k1 = c.x * p1, k2 = c.y * q1;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) gh[j] = s1 * (gh[j] - fmaf(xh[j], k2, k1));
+      for (int j = 0; j < 8; ++j) gh[j] = fmaf(xh[j], -s1 * k2, fmaf(gh[j], s1, -s1 * k1));
     }
     if (a.dx) {
       t.set(gh);
@@ -217,9 +217,30 @@ __global__ __launch_bounds__(NT, 2) void block_norm_bwd_k(BlkArgs a) {
   // dbeta1, dgate as far as they are there (nvec)
   float* p = a.part + (long)blockIdx.x * C;
   int v = 0;
+  // 4 columns of one vector a thread, all vectors at once
   auto drain = [&] {
     __syncthreads();
-    for (int k = 0; k < v; ++k, p += (long)gridDim.x * C) sum_cols<LPR, NT>(cols + k * col_floats<LPR, NT>(), tid, tpr, C, p);
+    const int quads = (C + 3) >> 2, jrows = col_rows<LPR, NT>(tpr), jcols = LPR < 64 ? LPR * 8 : tpr * 8;
+    for (int e = tid; e < v * quads; e += NT) {
+      const int k = e / quads, c = (e - k * quads) * 4;
+      const float* q = cols + k * col_floats<LPR, NT>() + c;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int r = 0; r < jrows; ++r) {
+        const float4 t = *(const float4*)(q + r * jcols);
+        s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+      }
+      float* o = p + (long)k * gridDim.x * C + c;
+      if (c + 4 <= C) {
+        __builtin_memcpy(o, &s, 16);
+      } else {
+        const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < C) o[j] = f[j];
+      }
+    }
+    p += (long)v * gridDim.x * C;
     v = 0;
   };
   auto flush = [&](float* acc, float mul) {

@@ -14,7 +14,7 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
   float* vecs = (float*)dyn;
   const int tid = threadIdx.x, tpr = LPR < 64 ? LPR : a.tpr, slots = NT / tpr, slot = tid / tpr;
   const int C = a.C, c0 = (tid % tpr) * 8;
-  const Lane<T, ALN> ln(slot, c0, C);
+  const Lane<T, ALN, LPR == 2> ln(slot, c0, C);
   const int nv = ln.nv, cc = nv ? c0 : 0;
   RowX rx;
   rx.init(xch, tid, NT, LPR, tpr, C);
@@ -42,8 +42,8 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
   while (r0 < a.M) {
     asm volatile("" ::: "memory");  // the column vectors stay in LDS
     float f[8], r[8], v[8], w[8];
-    nx.get(f);
-    nr.get(r);
+    ln.get(nx, f, on);
+    ln.get(nr, r, on);
     const long cur = r0, at = r0 * C;
     const uint32_t crows = rows;
     const bool con = on;
@@ -61,15 +61,11 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
       for (int j = 0; j < 8; ++j) f[j] = fmaf((f[j] - m1) * s1, v[j], w[j]);
     }
     if (a.gate_mode == GATE_GROUP) {
+      const Lane<T, false, LPR == 2> gl(0, c0, C);
+      gl.load(t, a.gate, (cur + slot) / a.rpg * C, 0, C, con);
+      gl.get(t, v, con);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
-      if (con) {
-        const Lane<T, false> gl(0, c0, C);
-        gl.load(t, a.gate, (cur + slot) / a.rpg * C, 0, C, true);
-        t.get(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= sc;
-      }
+      for (int j = 0; j < 8; ++j) v[j] *= sc;
     } else {
       cv.get(vecs, GV, v, cc, nv);
     }
@@ -111,12 +107,14 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
 }
 
 namespace {
+// Four waves a SIMD; three for rows above 1024 columns, which read more rows at a time as it is (32768 x 2048,
+// forward and backward together: 276 us with four, 259 with three; 401408 x 64: 56.9 with four, 58.2 with three).
 template <typename T, bool ALN, bool PO, bool PR, bool DROP>
 int fwd_launch(const BlkArgs& a, hipStream_t stream) {
   auto go = [&](auto kern, int nt, int tpr) {
     BlkArgs b = a;
     b.tpr = tpr;
-    const long slots = nt / tpr, wgs = (a.M + slots - 1) / slots, cap = 1024L * 256 / nt;  // four waves a SIMD
+    const long slots = nt / tpr, wgs = (a.M + slots - 1) / slots, cap = (a.C <= 1024 ? 1024L : 768L) * 256 / nt;
     kern<<<(int)(wgs < cap ? wgs : cap), nt, col_vec_bytes(nt, a.C, 5), stream>>>(b);
   };
   const int C = a.C;

@@ -14,7 +14,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._util import hip_on, on_device, ptr
+from ._util import hip_on, ptr
 
 GROUPS = (32, 64, 128)
 ACT = {None: 0, "linear": 0, "relu": 1}
@@ -161,7 +161,7 @@ def int4_workspace_floats(batch: int, w: Int4Weight) -> int:
 def int4_workspace(batch: int, w: Int4Weight) -> torch.Tensor | None:
     """Scratch of one product of ``batch`` rows (None where it needs none).  Products that may run at the
     same time - on two streams, or in two captured graphs - need one each."""
-    if not on_device(w.tiles):
+    if not w.tiles.is_cuda:
         return None
     n = int4_workspace_floats(batch, w)
     return torch.empty(n, dtype=torch.float32, device=w.tiles.device) if n else None
@@ -169,35 +169,47 @@ def int4_workspace(batch: int, w: Int4Weight) -> torch.Tensor | None:
 
 def int4_dense_fwd(x, w: Int4Weight, bias, act, out, workspace=None):
     """out[B, N] = act(x[B, K] @ w^T + bias): x bf16, bias fp32 [N] or None, act None / "linear" /
-    "relu", out bf16 or fp32."""
-    if act not in ACT:
+    "relu" (a NaN stays one), out bf16 or fp32, apart from x.  Infinities and NaN in x give what the formula
+    gives.  Sums are fp32; the order of a sum depends on the sizes alone."""
+    relu = ACT.get(act)
+    if relu is None:
         raise ValueError(f"int4_dense: activation {act!r}")
-    if x.dim() != 2 or x.shape[1] != w.k or not x.is_contiguous():
-        raise ValueError(f"int4_dense: x must be contiguous [batch, {w.k}]")
-    B, dev = x.shape[0], w.tiles.device
-    if tuple(out.shape) != (B, w.n) or not out.is_contiguous() or x.device != dev or out.device != dev:
-        raise ValueError(f"int4_dense: out must be contiguous [{B}, {w.n}], everything on {dev}")
-    if out.dtype not in (torch.bfloat16, torch.float32):
+    tiles, n, k = w.tiles, w.n, w.k
+    dev = tiles.device
+    if x.dim() != 2 or x.shape[1] != k or not x.is_contiguous():
+        raise ValueError(f"int4_dense: x must be contiguous [batch, {k}]")
+    B = x.shape[0]
+    if out.shape != (B, n) or not out.is_contiguous() or x.device != dev or out.device != dev:
+        raise ValueError(f"int4_dense: out must be contiguous [{B}, {n}], everything on {dev}")
+    f32 = out.dtype is torch.float32
+    if not f32 and out.dtype is not torch.bfloat16:
         raise TypeError(f"int4_dense: output {out.dtype}")
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (w.n,) or bias.device != dev
+    if bias is not None and (bias.dtype is not torch.float32 or bias.shape != (n,) or bias.device != dev
                              or not bias.is_contiguous()):
-        raise ValueError(f"int4_dense: bias must be a contiguous fp32 [{w.n}] on {dev}")
-    if not on_device(x):
+        raise ValueError(f"int4_dense: bias must be a contiguous fp32 [{n}] on {dev}")
+    if not tiles.is_cuda:
         y = x.float() @ int4_dequantize(w).t()
         if bias is not None:
             y = y + bias
-        out.copy_((torch.relu(y) if ACT[act] else y).to(out.dtype))
+        out.copy_((torch.relu(y) if relu else y).to(out.dtype))
         return out
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not torch.bfloat16:
         raise TypeError(f"int4_dense: x must be bfloat16, got {x.dtype}")
-    if x.data_ptr() & 15:
+    xp, op = x.data_ptr(), out.data_ptr()
+    if B and xp < op + B * n * (4 if f32 else 2) and op < xp + B * k * 2:
+        raise ValueError("int4_dense: out overlaps x")
+    if xp & 15:
         x = x.clone()  # the kernel reads 16 bytes at a time
+        xp = x.data_ptr()
     need = int4_workspace_floats(B, w)
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.float32, device=dev)
-    elif need and (workspace.dtype != torch.float32 or workspace.numel() < need or workspace.device != dev
-                   or not workspace.is_contiguous()):
-        raise ValueError(f"int4_dense: workspace must hold {need} contiguous floats on {dev}")
-    hip_on(dev, "ptg_int4_dense", ptr(x), ptr(w.tiles), ptr(w.scale), ptr(w.zero), ptr(bias), ptr(out), ptr(workspace), B,
-           w.n, w.k, w.group, ACT[act], int(out.dtype == torch.float32))
+    wp = None
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.float32, device=dev)
+        elif workspace.dtype is not torch.float32 or workspace.numel() < need or workspace.device != dev \
+                or not workspace.is_contiguous():
+            raise ValueError(f"int4_dense: workspace must hold {need} contiguous floats on {dev}")
+        wp = workspace.data_ptr()
+    hip_on(dev, "ptg_int4_dense", xp, tiles.data_ptr(), w.scale.data_ptr(), ptr(w.zero),
+           None if bias is None else bias.data_ptr(), op, wp, B, n, k, w.group, relu, f32)
     return out

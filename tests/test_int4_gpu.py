@@ -169,3 +169,6 @@ def test_refusals(hip_built):
     if Q.int4_workspace(1, w) is not None:
         with pytest.raises(ValueError):
             Q.int4_dense_fwd(x, w, None, None, out, workspace=torch.empty(5, device="cuda"))
+    both = torch.zeros(8192 + 8, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="overlaps"):
+        Q.int4_dense_fwd(both[:8192].view(1, 8192), w, None, None, both[4096:4608].view(1, 512))
