@@ -27,6 +27,8 @@ from __future__ import annotations
 import time
 
 import numpy as np
+import math
+
 import torch
 
 from . import engine as E
@@ -130,8 +132,9 @@ def _add_into(ex, g) -> None:
     if ex.dtype == g.dtype == torch.bfloat16:
         KB.add_(ex, g, ex)
     else:
-        NM.block_norm_fwd(g.to(ex.dtype).view(-1, g.shape[-1]), res=ex.view(-1, g.shape[-1]),
-                          h=ex.view(-1, g.shape[-1]))
+        rows = (-1, math.gcd(ex.numel(), NM.MAX_COLS))  # elementwise: any rows will do
+        ex = ex.view(rows)
+        NM.block_norm_fwd(g.to(ex.dtype).contiguous().view(rows), res=ex, h=ex)
 
 
 def _lower(nodes: list, input_idx: int) -> list:

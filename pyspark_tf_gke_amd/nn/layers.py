@@ -518,6 +518,13 @@ class _RowNorm(Layer):
 
     beta = None
 
+    def compute_output_shape(self, s):
+        from ..ops.norm import MAX_COLS
+
+        if s and s[-1] is not None and s[-1] > MAX_COLS:
+            raise NotImplementedError(f"{self.keras_class}: rows of at most {MAX_COLS} channels, got {s[-1]}")
+        return tuple(s)
+
     def _eps(self, epsilon):
         if not float(epsilon) > 0.0:
             raise ValueError(f"{self.keras_class}: epsilon must be positive, got {epsilon}")

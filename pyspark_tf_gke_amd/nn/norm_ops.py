@@ -8,6 +8,8 @@ draws the dropout mask again instead of reading one.  Any part alone is the same
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from ..ops import dropout as DR
@@ -165,8 +167,27 @@ class BlockOp:
         self._kw = dict(res=res, post=self._norm(self.post), gate=gate, scale=self.scale, drop=d,
                         pre=self._norm(self.pre))
         self._x, self._st, self._gshape = x, st, xs[1].shape if self.gate_input else None
-        NM.block_norm_fwd(x, h=h, u=u, stats=st, **self._kw)
+        if self._wide(x):
+            if st is not None:
+                self._st = ws.get(self.name + "/stats", (4, self._flat(x).shape[0]), torch.float32, dev)
+            kw = self._wide_kw()
+            NM.block_norm_fwd(self._flat(x), h=self._flat(h), stats=self._st, **kw)
+        else:
+            NM.block_norm_fwd(x, h=h, u=u, stats=st, **self._kw)
         return [t for t in (h, u) if t is not None]
+
+    # Rows above the kernels' width, without a norm or a gate vector: elementwise, so any rows will do
+    # (the dropout mask goes by the element's index).
+    def _wide(self, x) -> bool:
+        return x.shape[-1] > NM.MAX_COLS and self.post is None and self.pre is None and self.gate is None \
+            and (not self.gate_input or self._kw["gate"].numel() == x.numel())
+
+    @staticmethod
+    def _flat(t):
+        return None if t is None else t.view(-1, math.gcd(t.numel(), NM.MAX_COLS))
+
+    def _wide_kw(self):
+        return {**self._kw, "res": self._flat(self._kw["res"]), "gate": self._flat(self._kw["gate"])}
 
     def _grads(self, layer):
         if layer is None:
@@ -196,13 +217,16 @@ class BlockOp:
         elif self.gate is not None:
             dgate = self.gate.gamma.grad
         wsp = None
+        fl = lambda t: t  # noqa: E731
+        if self._wide(x):
+            fl, kw = self._flat, self._wide_kw()
         if x.is_cuda:
-            C = x.shape[-1]
+            C = fl(x).shape[-1]
             M = x.numel() // C
             G = kw["gate"].shape[0] if self.gate_input else 1
             wsp = ws.get(self.name + "/colsums", (NM.block_norm_workspace_floats(M, C, G),), torch.float32, dev)
-        NM.block_norm_bwd(x, st, du=du, dh=dh, dx=dx, dres=dres, dgate=dgate, dpost=self._grads(self.post),
-                          dpre=self._grads(self.pre), workspace=wsp, **kw)
+        NM.block_norm_bwd(fl(x), st, du=du, dh=fl(dh), dx=fl(dx), dres=fl(dres), dgate=fl(dgate),
+                          dpost=self._grads(self.post), dpre=self._grads(self.pre), workspace=wsp, **kw)
         return [dx] + ([dgate.view(self._gshape)] if self.gate_input else []) + ([dres] if self.res else [])
 
 

@@ -301,3 +301,41 @@ def test_model_checker_answers_from_4_bits(tmp_path):
                         str(tmp_path), "--model", path, "--images", str(imgs), "--device", "cpu", "--quantize", "int4"],
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "predicted (x=" in r.stdout, r.stderr[-2000:]
+
+
+def wide_model(width, device="cpu"):
+    """Residual scales, dropout and a gate of the branch's shape over rows wider than the kernels' 8192."""
+    L.reset_name_counters()
+    inp = nn.Input(shape=(24,))
+    h = nn.Dense(width, name="stem")(inp)
+    g = nn.Dense(width, name="cond")(inp)
+    y = nn.Dropout(0.2, name="drop")(nn.Rescaling(0.5, name="half")(nn.Multiply(name="gate")([h, g])))
+    m = nn.Model(inp, nn.Dense(2, name="head")(nn.Add(name="sum")([h, y])))
+    m.build(device=device)
+    m.compile(optimizer=nn.optimizers.SGD(0.0), loss="mse")
+    return m
+
+
+@pytest.mark.parametrize("width", [8200, 16384])
+def test_wide_rows_without_a_norm(fp32_host, width):
+    m = wide_model(width)
+    assert any(isinstance(op, NO.BlockNode) and op.op.drop is not None and op.op.res for op in m.ops)
+    agree(m, *data(3, 24), 1, 5e-5)
+
+
+def test_norms_refuse_wide_rows():
+    wide = nn.Input(shape=(8200,)).output
+    for layer in (nn.LayerNormalization(), nn.RMSNormalization(), nn.LayerScale()):
+        with pytest.raises(NotImplementedError, match="8192"):
+            layer(wide)
+    with pytest.raises(NotImplementedError, match="8192"):
+        nn.Sequential([nn.Input(shape=(8200,)), nn.LayerNormalization(), nn.Dense(2)]).build(device="cpu")
+
+
+def test_fp32_gradients_of_wide_rows_add():
+    from pyspark_tf_gke_amd.nn.functional import _add_into
+
+    a, b = torch.randn(3, 9001), torch.randn(3, 9001)
+    want = a + b
+    _add_into(a, b)
+    assert torch.equal(a, want)

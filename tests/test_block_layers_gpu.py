@@ -8,7 +8,7 @@ import block_oracle as BO
 from pyspark_tf_gke_amd import nn
 from pyspark_tf_gke_amd.models import build_cnn_model, build_deep_model
 from pyspark_tf_gke_amd.nn import norm_ops as NO
-from test_block_layers_cpu import data, engine_grads, tower
+from test_block_layers_cpu import data, engine_grads, tower, wide_model
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,26 @@ def test_mlp_with_dropout(hip_built):
 
 
 _ = torch
+
+
+@pytest.mark.parametrize("width", [8200, 16384])
+def test_wide_rows_without_a_norm(hip_built, width):
+    m = wide_model(width, device="cuda")
+    x, y = data(37, 24)
+    for step in (1, 2):
+        out, g = engine_grads(m, x, y)
+        spread = {}
+        want, _, ref = BO.run(m, x, y, step, spread=spread)
+        assert float((out - want).norm() / want.norm()) < OUT_TOL
+        for name, r in ref.items():
+            assert float((g[name] - r).norm() / (r.norm() + spread[name].norm())) < GRAD_TOL, name
+
+
+def test_fp32_gradients_of_wide_rows_add(hip_built):
+    from pyspark_tf_gke_amd.nn.functional import _add_into
+
+    for dt in (torch.float32, torch.bfloat16):
+        a, b = torch.randn(5, 20480, device="cuda"), torch.randn(5, 20480, device="cuda").to(dt)
+        want = a + b.float()
+        _add_into(a, b)
+        assert torch.equal(a, want)
