@@ -121,6 +121,16 @@ static inline FastDiv fastdiv(uint32_t d) {
   return f;
 }
 
+// Lets `kernel` take `bytes` of dynamic LDS (above 64 KB) on the current device; `done` keeps the devices
+// where that is set (setting it twice is harmless).
+static inline void ptg_allow_lds(const void* kernel, int bytes, uint64_t& done) {
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  if (dev < 64 && (done >> dev & 1)) return;
+  (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (dev < 64) done |= 1ull << dev;
+}
+
 #define PTG_RETURN_LAUNCH() return (int)hipGetLastError()
 
 // Workgroups of `kernel` (256 threads) resident at once on the whole device: the grid of a

@@ -344,11 +344,8 @@ template <typename T, int LPR, int NT, bool ALN, bool PO, bool PR, bool GG, bool
 void bwd_run(const BlkArgs& a, int grid, hipStream_t st) {
   auto kern = block_norm_bwd_k<T, LPR, NT, ALN, PO, PR, GG, DROP>;
   const int lds = col_vec_bytes(NT, a.C, 4) + flush_vecs<NT>() * col_floats<LPR, NT>() * 4;
-  static bool set = false;  // setting it twice is harmless
-  if (LPR == 64 && !set) {
-    (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
-    set = true;
-  }
+  static uint64_t set = 0;  // devices whose limit is raised
+  if (LPR == 64) ptg_allow_lds((const void*)kern, 128 * 1024, set);
   kern<<<grid, NT, lds, st>>>(a);
 }
 template <typename T, bool ALN, bool PO, bool PR, bool GG, bool DROP>

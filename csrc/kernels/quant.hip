@@ -436,11 +436,8 @@ template <int GS>
 void go4t(const Plan4& p, const Args4& a, hipStream_t st) {
   auto kern = a.z ? int4_tile_k<GS, true> : int4_tile_k<GS, false>;
   constexpr int lds = QR * Q_STAGE;
-  static bool set[2];  // of these two kernels; setting it twice is harmless
-  if (!set[a.z != nullptr]) {
-    (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    set[a.z != nullptr] = true;
-  }
+  static uint64_t set[2];  // devices whose limit is raised, for each of the two kernels
+  ptg_allow_lds((const void*)kern, lds, set[a.z != nullptr]);
   kern<<<p.mb * p.nb * p.splits, 512, lds, st>>>(a, p.mb, p.nb, p.splits);
 }
 template <int GS>

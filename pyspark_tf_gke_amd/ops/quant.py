@@ -93,18 +93,20 @@ def int4_layout(codes, scale, zero=None, group: int = 128) -> Int4Weight:
     if zero is not None and int(zero.max()) > 15:
         raise ValueError("int4: zero points must lie in 0..15")
     Np, Kp = -(-N // 16) * 16, -(-K // 128) * 128
-    q = torch.zeros((Np, Kp), dtype=torch.int64, device=codes.device)
-    q[:N, 0:K:2] = (codes & 15).long()
-    q[:N, 1:K:2] = (codes >> 4).long()
-    # [nt, n, kt, i, quarter, s, odd]: input kt*128 + i*32 + quarter*8 + 2*s + odd -> nibble s + 4*odd of
-    # dword i of lane quarter*16 + n
-    q = q.view(Np // 16, 16, Kp // 128, 4, 4, 4, 2)
-    sh = (4 * (torch.arange(4, device=q.device)[:, None] + 4 * torch.arange(2, device=q.device)[None, :]))
-    words = (q << sh).sum((5, 6))  # [nt, n, kt, i, quarter]
-    words = ((words << 3) | (words >> 29)) & 0xFFFFFFFF
-    words = words.permute(0, 2, 4, 1, 3).reshape(Np // 16, Kp // 128, 64, 4)  # [nt, kt, lane, dword]
-    tiles = torch.stack([(words >> (8 * b)) & 0xFF for b in range(4)], -1).to(torch.uint8)
-    tiles = tiles.reshape(Np // 16, Kp // 128, 64, 16).contiguous()
+    if (Np, Kp) != (N, K) or not codes.is_contiguous() or codes.storage_offset() % 4:
+        padded = torch.zeros((Np, Kp // 2), dtype=torch.uint8, device=codes.device)
+        padded[:N, : K // 2] = codes
+        codes = padded
+    # a dword of 8 inputs: the even ones' nibbles in its low half, the odd ones' in its high half, rotated
+    v = codes.view(torch.int32)
+    half = [v & 0x0F0F0F0F, (v >> 4) & 0x0F0F0F0F]
+    half = [(h | (h >> 4)) & 0x00FF00FF for h in half]
+    half = [(h | (h >> 8)) & 0xFFFF for h in half]
+    words = half[0] | (half[1] << 16)
+    words = (words << 3) | ((words >> 29) & 7)
+    # [nt, n, kt, i, quarter] -> dword i of lane quarter * 16 + n
+    words = words.view(Np // 16, 16, Kp // 128, 4, 4).permute(0, 2, 4, 1, 3).contiguous()
+    tiles = words.view(torch.uint8).reshape(Np // 16, Kp // 128, 64, 16)
 
     def group_rows(t):
         if t is None:
@@ -176,6 +178,11 @@ def int4_dense_fwd(x, w: Int4Weight, bias, act, out, workspace=None):
         raise ValueError(f"int4_dense: activation {act!r}")
     tiles, n, k = w.tiles, w.n, w.k
     dev = tiles.device
+    groups = tiles.numel() * 2 // w.group
+    if tiles.numel() != (n + 15) // 16 * ((k + 127) // 128) * 1024 or w.scale.numel() != groups \
+            or w.scale.device != dev or (w.zero is not None and (w.zero.numel() != groups or w.zero.device != dev)):
+        raise ValueError(f"int4_dense: the weight is not what int4_layout gives for [{n}, {k}], groups of {w.group}, on "
+                         "one device")
     if x.dim() != 2 or x.shape[1] != k or not x.is_contiguous():
         raise ValueError(f"int4_dense: x must be contiguous [batch, {k}]")
     B = x.shape[0]

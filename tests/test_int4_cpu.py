@@ -102,6 +102,27 @@ def test_refusals():
         (lambda: Q.int4_dense_fwd(x, w, None, None, torch.empty(2, 5)), ValueError),
         (lambda: Q.int4_dense_fwd(x, w, None, None, torch.empty(2, 4, dtype=torch.float16)), TypeError),
         (lambda: Q.int4_dense_fwd(x, w, torch.zeros(5), None, out), ValueError),
+        (lambda: Q.int4_dense_fwd(x, w._replace(n=20), None, None, torch.empty(2, 20)), ValueError),
+        (lambda: Q.int4_dense_fwd(x, w._replace(scale=w.scale[:, :, :8]), None, None, out), ValueError),
+        (lambda: Q.int4_dense_fwd(x, w._replace(group=32), None, None, out), ValueError),
     ]:
         with pytest.raises(exc):
             call()
+
+
+def test_layout_of_views():
+    """Codes that are a slice of something, at any byte, lay out like a copy of their own."""
+    codes, scale, z, _ = codes_for(20, 256, 64, True)
+    want = Q.int4_layout(codes, scale, z, 64)
+    flat = torch.zeros(20 * 128 + 3, dtype=torch.uint8)
+    flat[3:] = codes.reshape(-1)
+    wide = torch.zeros(20, 140, dtype=torch.uint8)
+    wide[:, 5:133] = codes
+    for v in (flat[3:].view(20, 128), wide[:, 5:133]):
+        got = Q.int4_layout(v, scale, z, 64)
+        assert torch.equal(got.tiles, want.tiles) and got.tiles.is_contiguous()
+    codes16, scale16, _, _ = codes_for(16, 128, 128, False)  # a full tile: nothing to pad
+    w = Q.int4_layout(codes16, scale16, None, 128)
+    assert torch.equal(Q.int4_codes(w)[0], codes16)
+    codes16.fill_(0)
+    assert Q.int4_codes(w)[0].any()  # a copy, not a view
