@@ -77,7 +77,7 @@ PTG_DEV void int4_finish(const Args4& a, int m, int n, float s) {
 
 }  // namespace
 
-// Up to 32 rows: bound by reading the weights once.  A wave computes 16 * MT rows x 16 * NT outputs over its
+// Up to 32 rows, and small products: bound by reading the weights once.  A wave computes 16 * MT rows x 16 * NT outputs over its
 // share of K; the NW waves of a workgroup take the tiles of the workgroup's K range in turn and are joined
 // in LDS in a fixed order.  A product tile is one MFMA chain: sum (16 + u) x on top of -(16 + z) * sum x,
 // the latter from one MFMA with ones for every 32 inputs that all NT tiles share.  Waves that need few
@@ -91,12 +91,13 @@ struct Group {  // of a tile: 4 / GS groups
   uint8_t z[NG];
 };
 template <int MT, int NT, int NW, int GS, bool HASZ>
-__global__ __launch_bounds__(NW * 64) void int4_mm_k(Args4 a) {
+__global__ __launch_bounds__(NW * 64) void int4_mm_k(Args4 a, int splits) {
   constexpr int NG = 4 / GS, R = MT * NT * 4;
   constexpr bool FLAT = R * NW <= 128;  // every wave's sums in LDS at once, else pairwise
   __shared__ float red[(FLAT ? NW : NW / 2) * R][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, q = lane >> 4;
-  const int sp = blockIdx.x, splits = gridDim.x, nb = blockIdx.y * NT, m0 = blockIdx.z * 16 * MT;
+  const int nbi = splits == 1 ? blockIdx.x : blockIdx.x / splits, sp = blockIdx.x - nbi * splits;
+  const int nb = nbi * NT, m0 = blockIdx.y * 16 * MT;
   const int M = a.M, N = a.N, K = a.K, kt = a.kt, ntiles = (N + 15) / 16;
   const int t0 = (int)((long)kt * sp / splits), t1 = (int)((long)kt * (sp + 1) / splits);
   // rows, tiles of outputs and inputs that do not exist read 0
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(NW * 64) void int4_mm_k(Args4 a) {
   }
 }
 
-// Batches of more than 32 rows are bound by the matrix cores and by what feeds them, not by HBM.  A workgroup
+// Larger products of more than 32 rows are bound by the matrix cores and by what feeds them, not by HBM.  A workgroup
 // takes 64 rows x 256 outputs; 4 waves hold 64 x 64 of them each, twice over: waves 4..7 work on every
 // other stage of 128 inputs, so two waves share a SIMD and one multiplies while the other waits, and the
 // two halves are added at the end.  A stage (64 rows of inputs, 16 KB, and 16 weight tiles, 16 KB) goes
@@ -396,41 +397,47 @@ __global__ __launch_bounds__(256) void int4_join_k(Args4 a, int splits) {
 
 namespace {
 constexpr int Q_NW = 16;  // waves of int4_mm_k
-// Above 32 rows the tile kernel: 32 x 8192 x 8192 measured 19.3 us with it and 22.9 without, but 32 x 2048 x
-// 20480 20.6 and 17.8, 12 x 8192 x 8192 17.3 and 12.1.
-//
 // Outputs alone give one workgroup a CU only where N is large; otherwise K is split, up to one workgroup a
 // CU (two: 16 x 8192 x 8192 17.0 instead of 13.4 us, 12 x 2048 x 20480 13.9 instead of 10.9).  A split costs
 // the join, about 2.2 us, so a wave keeps at least 4 tiles (one row: 4 x 2048 x 8192 7.2 us whole, 9.4 in two)
 // or 2 where it works on two columns of tiles at a time (12 x 2048 x 20480 10.9 us in four, 22.5 whole).
+//
+// Above 32 rows the tile kernel, unless int4_mm_k is through after `steps` = 2 tiles of a wave (4 for groups
+// below 128, whose sums cost the tile kernel more): 128 x 1024 x 1024 (1 step) 7.4 instead of 12.0 us, 256 x 2048
+// x 2048 (2) 16.3 instead of 16.7, 128 x 8192 x 1024 (4) 18.9 instead of 16.1, 64 x 8192 x 8192 (8) 40.1 instead of
+// 22.4; groups of 32, 256 x 1024 x 4096 (2) 13.9 instead of 19.1, 128 x 2048 x 8192 (4) 22.4 instead of 23.8, 256 x
+// 8192 x 512 (8) 39.8 instead of 17.0.  Up to 32 rows it has the fewer rows for its 64: 12 x 8192 x 8192
+// 17.3 instead of 12.1 us.
 struct Plan4 { int tile, mt, nt, mb, nb, splits; };
-Plan4 plan4(int M, int N, int K) {
+Plan4 plan4(int M, int N, int K, int group) {
   Plan4 p;
   const long kt = (K + QT_K - 1) / QT_K;
-  p.tile = M > 32;
-  long least;  // tiles of a split at least
-  if (p.tile) {
+  p.tile = 0;
+  p.mt = M <= 16 ? 1 : 2;
+  p.nt = M <= 8 ? 1 : 2;  // two: half the reads of the inputs; 16 x 8192 x 8192 13.4 us instead of 19.5
+  p.mb = (M + 16 * p.mt - 1) / (16 * p.mt);
+  p.nb = (N + 16 * p.nt - 1) / (16 * p.nt);
+  const long least = Q_NW * (p.nt == 1 ? 4 : 2);  // tiles of a split
+  long wgs = (long)p.nb * p.mb, s = (256 + wgs - 1) / wgs;
+  s = s < kt / least ? s : kt / least;
+  s = s < 1 ? 1 : s;
+  const long steps = (wgs * s + 255) / 256 * ((kt + s * Q_NW - 1) / (s * Q_NW));
+  if (M > 32 && steps > (group == 128 ? 2 : 4)) {
+    p.tile = 1;
     p.mb = (M + QT_M - 1) / QT_M;
     p.nb = (N + QT_N - 1) / QT_N;
-    least = 4;
-  } else {
-    p.mt = M <= 16 ? 1 : 2;
-    p.nt = M <= 8 ? 1 : 2;  // two: half the reads of the inputs; 16 x 8192 x 8192 13.4 us instead of 19.5
-    p.mb = (M + 16 * p.mt - 1) / (16 * p.mt);
-    p.nb = (N + 16 * p.nt - 1) / (16 * p.nt);
-    least = Q_NW * (p.nt == 1 ? 4 : 2);
+    wgs = (long)p.nb * p.mb;
+    s = 256 / wgs < kt / 4 ? 256 / wgs : kt / 4;
+    s = s < 1 ? 1 : s;
   }
-  const long wgs = (long)p.nb * p.mb;
-  long s = p.tile ? 256 / wgs : (256 + wgs - 1) / wgs;
-  if (s > kt / least) s = kt / least;
-  p.splits = s < 1 ? 1 : (int)s;
+  p.splits = (int)s;
   return p;
 }
 template <int MT, int NT, int NW, int GS>
 void go4(const Plan4& p, const Args4& a, hipStream_t st) {
-  const dim3 grid(p.splits, p.nb, p.mb);
-  if (a.z) int4_mm_k<MT, NT, NW, GS, true><<<grid, NW * 64, 0, st>>>(a);
-  else int4_mm_k<MT, NT, NW, GS, false><<<grid, NW * 64, 0, st>>>(a);
+  const dim3 grid((unsigned)p.splits * p.nb, p.mb);
+  if (a.z) int4_mm_k<MT, NT, NW, GS, true><<<grid, NW * 64, 0, st>>>(a, p.splits);
+  else int4_mm_k<MT, NT, NW, GS, false><<<grid, NW * 64, 0, st>>>(a, p.splits);
 }
 template <int GS>
 void go4t(const Plan4& p, const Args4& a, hipStream_t st) {
@@ -458,8 +465,8 @@ int go4g(const Plan4& p, const Args4& a, hipStream_t st) {
 extern "C" {
 
 // *floats: workspace of a product of M rows (0 where none is needed)
-int ptg_int4_ws(int M, int N, int K, void* floats) {
-  const int splits = M > 0 ? plan4(M, N, K).splits : 1;
+int ptg_int4_ws(int M, int N, int K, int group, void* floats) {
+  const int splits = M > 0 ? plan4(M, N, K, group).splits : 1;
   *(long*)floats = splits > 1 ? (long)splits * M * N : 0;
   return 0;
 }
@@ -471,7 +478,7 @@ int ptg_int4_dense(const void* x, const void* w, const void* scale, const void* 
   // a block of rows or of outputs stays below 2 GiB
   if ((group != 32 && group != 64 && group != 128) || K < group || K % group || K > (1 << 22) || ((uintptr_t)x & 15))
     return (int)hipErrorInvalidValue;
-  const Plan4 p = plan4(M, N, K);
+  const Plan4 p = plan4(M, N, K, group);
   if (p.splits > 1 && !ws) return (int)hipErrorInvalidValue;
   const Args4 a{(const bf16_t*)x, (const uint8_t*)w, (const bf16_t*)scale, (const uint8_t*)zero, (const float*)bias,
                 y, p.splits > 1 ? (float*)ws : nullptr, M, N, K, (K + QT_K - 1) / QT_K, act, f32};

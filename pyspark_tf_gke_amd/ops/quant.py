@@ -147,13 +147,13 @@ _WS: dict = {}
 
 def int4_workspace_floats(batch: int, w: Int4Weight) -> int:
     """Floats of :func:`int4_workspace`."""
-    key = (batch, w.n, w.k)
+    key = (batch, w.n, w.k, w.group)
     v = _WS.get(key)
     if v is None:
         from .. import _native
 
         n = ctypes.c_long(0)
-        _native.check(_native.hip_lib().ptg_int4_ws(batch, w.n, w.k, ctypes.byref(n)), "ptg_int4_ws")
+        _native.check(_native.hip_lib().ptg_int4_ws(batch, w.n, w.k, w.group, ctypes.byref(n)), "ptg_int4_ws")
         if len(_WS) > 4096:
             _WS.clear()
         v = _WS[key] = n.value

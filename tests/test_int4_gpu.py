@@ -17,7 +17,8 @@ def weights64(codes, scale, zero, group):
 SHAPES = [(1, 1, 32, 32), (1, 16, 128, 128), (3, 17, 160, 32), (5, 33, 320, 64), (16, 100, 1024, 128),
           (17, 48, 2048, 64), (1, 2048, 20480, 128), (2, 7, 4096, 32), (33, 130, 1280, 128), (64, 64, 512, 64),
           (65, 50, 1056, 32), (130, 300, 2560, 128), (256, 64, 640, 64), (300, 272, 1152, 128), (1, 5000, 256, 64),
-          (70, 530, 3040, 32), (40, 256, 20480, 64), (129, 1000, 4160, 64)]
+          (70, 530, 3040, 32), (40, 256, 20480, 64), (129, 1000, 4160, 64), (33, 2, 32, 32), (70, 8200, 1056, 32),
+          (64, 8192, 1280, 128), (255, 3100, 960, 64), (1, 1 << 21, 32, 32)]
 
 
 @pytest.mark.parametrize("B,N,K,group", SHAPES)
