@@ -27,6 +27,30 @@ struct BlkArgs {
   int C, tpr, slotwise, sub, nvec;
 };
 
+// Arguments of the C entries, one block of 64-bit fields (a call with as many arguments of its own costs the
+// host about 2 us more).  Addresses of tensors that are not there are 0.
+struct FwdCall {
+  const void *x, *res, *gate;
+  void *h, *u;
+  const float *g1, *b1, *g2, *b2;
+  float* stats;
+  const void* step_dev;
+  int64_t M, C, f32, aligned, kind1, kind2, gate_mode, rpg, drop, thr, seed, step;
+  double eps1, eps2, scale, dscale;
+};
+struct BwdCall {
+  const void *x, *res, *gate, *du, *dh;
+  void *dx, *dres;
+  const float *g1, *b1, *g2;
+  float *stats, *dg1, *db1, *dg2, *db2;
+  void* dgate;
+  float* ws;
+  const void* step_dev;
+  int64_t M, C, f32, aligned, kind1, kind2, gate_mode, rpg, drop, thr, seed, step;
+  double scale, dscale;
+};
+static_assert(sizeof(FwdCall) == 27 * 8 && sizeof(BwdCall) == 32 * 8, "64-bit fields");
+
 typedef __attribute__((ext_vector_type(4))) unsigned int vu4_t;
 
 // ---- sums over the LPR lanes of a row (every lane gets the sum) --------------------------------

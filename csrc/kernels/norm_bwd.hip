@@ -323,20 +323,20 @@ Shape shape_of(int C) {
   if (C <= 2048) return {64, 512, 256};
   return {64, 1024, C <= 4096 ? 512 : 1024};
 }
-// Work items: bundles of `slots` groups while groups are short; a long group is an item of its own, or
-// is split (`sub`) where there are too few groups to fill the workgroups.
+// Work items: bundles of `slots` groups, each slot going through a group of its own; or a long group is an
+// item whose rows the slots share, split (`sub`) where there are too few groups to fill the workgroups.
+// The fewer rows one after another win; an item of shared rows ends in a join, worth about two rows (62 x 24, one
+// group: 90 us as 62 rows of one slot).  Slots of long groups would stand too far apart for 32-bit offsets.
 void plan(BlkArgs& a, const Shape& s, int& grid) {
   const long slots = s.nt / s.tpr, G = a.M / a.rpg;
-  a.slotwise = a.rpg <= 4 * slots || a.rpg <= 16;
-  a.sub = 1;
-  if (a.slotwise) {
-    a.items = (G + slots - 1) / slots;
-  } else {
-    const long want = BWD_WGS / (G < BWD_WGS ? G : BWD_WGS), most = a.rpg / slots;
-    a.sub = (int)(want < most ? want : most);
-    if (a.sub < 1) a.sub = 1;
-    a.items = G * a.sub;
-  }
+  auto up = [](long x, long y) { return (x + y - 1) / y; };
+  const long want = BWD_WGS / (G < BWD_WGS ? G : BWD_WGS), most = a.rpg / slots;
+  const long sub = most < 1 ? 1 : want < most ? want : most;
+  const long own = up(up(G, slots), BWD_WGS) * a.rpg;
+  const long shared = up(G * sub, BWD_WGS) * (up(up(a.rpg, sub), slots) + 2);
+  a.slotwise = a.rpg <= (4 * slots > 16 ? 4 * slots : 16) && own <= shared;
+  a.sub = a.slotwise ? 1 : (int)sub;
+  a.items = a.slotwise ? up(G, slots) : G * sub;
   grid = (int)(a.items < BWD_WGS ? a.items : BWD_WGS);
 }
 
@@ -396,20 +396,23 @@ int ptg_block_norm_ws(long M, int C, long groups, void* floats) {
   return 0;
 }
 
-int ptg_block_norm_bwd(const void* x, const void* res, const void* gate, const void* du, const void* dh, void* dx,
-                       void* dres, const void* g1, const void* b1, const void* g2, const void* stats, void* dg1,
-                       void* db1, void* dg2, void* db2, void* dgate, void* ws, long M, int C, int f32, int aligned,
-                       int kind1, int kind2, int gate_mode, long rpg, float scale, int drop, int thr, float dscale,
-                       long seed, long step, const void* step_dev, hipStream_t stream) {
+// call: a BwdCall, `aligned` and `rpg` as in the forward pass
+int ptg_block_norm_bwd(const void* call, hipStream_t stream) {
+  const BwdCall& c = *(const BwdCall*)call;
+  const long M = c.M, rpg = c.rpg;
+  const int C = (int)c.C, kind1 = (int)c.kind1, kind2 = (int)c.kind2, gate_mode = (int)c.gate_mode;
+  const bool f32 = c.f32, aligned = c.aligned;
+  float *dg1 = c.dg1, *db1 = c.db1, *dg2 = c.dg2, *db2 = c.db2;
+  void *dgate = c.dgate, *ws = c.ws;
   if (M <= 0) return 0;
-  if (C < 1 || C > 8192 || (gate_mode == GATE_GROUP && (rpg < 1 || M % rpg))) return (int)hipErrorInvalidValue;
+  if (c.C < 1 || c.C > 8192 || (gate_mode == GATE_GROUP && (rpg < 1 || M % rpg))) return (int)hipErrorInvalidValue;
   BlkArgs a{};
-  a.x = x; a.res = res; a.gate = gate; a.du = du; a.dh = dh; a.dx = dx; a.dres = dres;
-  a.g1 = (const float*)g1; a.b1 = (const float*)b1; a.g2 = (const float*)g2;
-  a.stats = (float*)stats;
+  a.x = c.x; a.res = c.res; a.gate = c.gate; a.du = c.du; a.dh = c.dh; a.dx = c.dx; a.dres = c.dres;
+  a.g1 = c.g1; a.b1 = c.b1; a.g2 = c.g2;
+  a.stats = c.stats;
   a.M = M; a.C = C; a.kind1 = kind1; a.kind2 = kind2;
-  a.gate_mode = gate_mode; a.rpg = gate_mode == GATE_GROUP ? rpg : 1; a.scale = scale; a.drop = drop;
-  a.d = drop_args(thr, dscale, seed, step, step_dev);
+  a.gate_mode = gate_mode; a.rpg = gate_mode == GATE_GROUP ? rpg : 1; a.scale = (float)c.scale; a.drop = (int)c.drop;
+  a.d = drop_args((int)c.thr, (float)c.dscale, c.seed, c.step, c.step_dev);
   a.dgate = dgate;
   const Shape s = shape_of(C);
   int grid;
@@ -417,12 +420,12 @@ int ptg_block_norm_bwd(const void* x, const void* res, const void* gate, const v
   a.tpr = s.tpr;
   ColSums cs{};
   if (kind2) {
-    cs.dst[a.nvec++] = (float*)dg2;
-    if (kind2 == NORM_LAYER) cs.dst[a.nvec++] = (float*)db2;
+    cs.dst[a.nvec++] = dg2;
+    if (kind2 == NORM_LAYER) cs.dst[a.nvec++] = db2;
   }
   if (kind1) {
-    cs.dst[a.nvec++] = (float*)dg1;
-    if (kind1 == NORM_LAYER) cs.dst[a.nvec++] = (float*)db1;
+    cs.dst[a.nvec++] = dg1;
+    if (kind1 == NORM_LAYER) cs.dst[a.nvec++] = db1;
   }
   if (gate_mode == GATE_VEC) cs.dst[a.nvec++] = (float*)dgate;
   a.part = (float*)ws;

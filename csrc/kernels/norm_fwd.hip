@@ -138,23 +138,21 @@ int fwd_drop(const BlkArgs& a, hipStream_t stream) {
 
 extern "C" {
 
-// aligned: every tensor starts on 16 bytes and C % 8 == 0.  Rows per gate group: rpg.
-int ptg_block_norm_fwd(const void* x, const void* res, const void* gate, void* h, void* u, const void* g1,
-                       const void* b1, const void* g2, const void* b2, void* stats, long M, int C, int f32,
-                       int aligned, int kind1, float eps1, int kind2, float eps2, int gate_mode, long rpg, float scale,
-                       int drop, int thr, float dscale, long seed, long step, const void* step_dev,
-                       hipStream_t stream) {
-  if (M <= 0) return 0;
-  if (C < 1 || C > 8192) return (int)hipErrorInvalidValue;
+// call: a FwdCall.  aligned: every tensor starts on 16 bytes and C % 8 == 0.  Rows per gate group: rpg.
+int ptg_block_norm_fwd(const void* call, hipStream_t stream) {
+  const FwdCall& c = *(const FwdCall*)call;
+  if (c.M <= 0) return 0;
+  if (c.C < 1 || c.C > 8192) return (int)hipErrorInvalidValue;
   BlkArgs a{};
-  a.x = x; a.res = res; a.gate = gate; a.h = h; a.u = u;
-  a.g1 = (const float*)g1; a.b1 = (const float*)b1; a.g2 = (const float*)g2; a.b2 = (const float*)b2;
-  a.stats = (float*)stats;
-  a.M = M; a.C = C; a.kind1 = kind1; a.kind2 = kind2; a.eps1 = eps1; a.eps2 = eps2;
-  a.gate_mode = gate_mode; a.rpg = rpg > 0 ? rpg : 1; a.scale = scale; a.drop = drop;
-  a.d = drop_args(thr, dscale, seed, step, step_dev);
-  if (f32) return aligned ? fwd_drop<float, true>(a, stream) : fwd_drop<float, false>(a, stream);
-  return aligned ? fwd_drop<bf16_t, true>(a, stream) : fwd_drop<bf16_t, false>(a, stream);
+  a.x = c.x; a.res = c.res; a.gate = c.gate; a.h = c.h; a.u = c.u;
+  a.g1 = c.g1; a.b1 = c.b1; a.g2 = c.g2; a.b2 = c.b2;
+  a.stats = c.stats;
+  a.M = c.M; a.C = (int)c.C; a.kind1 = (int)c.kind1; a.kind2 = (int)c.kind2;
+  a.eps1 = (float)c.eps1; a.eps2 = (float)c.eps2;
+  a.gate_mode = (int)c.gate_mode; a.rpg = c.rpg > 0 ? c.rpg : 1; a.scale = (float)c.scale; a.drop = (int)c.drop;
+  a.d = drop_args((int)c.thr, (float)c.dscale, c.seed, c.step, c.step_dev);
+  if (c.f32) return c.aligned ? fwd_drop<float, true>(a, stream) : fwd_drop<float, false>(a, stream);
+  return c.aligned ? fwd_drop<bf16_t, true>(a, stream) : fwd_drop<bf16_t, false>(a, stream);
 }
 
 }  // extern "C"

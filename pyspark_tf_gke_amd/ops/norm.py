@@ -19,15 +19,21 @@ GPU tensors run the kernels, CPU tensors the fp32 reference below.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
 
 from . import dropout as DR
-from ._util import hip_on, ptr
+from ._util import hip_on
 
 KINDS = {"layer": 1, "rms": 2}
 MAX_COLS = 8192
+
+
+# arguments of the C entries: 64 bits each, as FwdCall and BwdCall of norm.h
+_FWD = struct.Struct("=11Q12q4d")
+_BWD = struct.Struct("=18Q12q2d")
 
 
 class Norm(NamedTuple):
@@ -57,7 +63,7 @@ def block_norm_workspace(rows: int, cols: int, groups: int, device) -> torch.Ten
     return torch.empty(block_norm_workspace_floats(rows, cols, groups), dtype=torch.float32, device=device)
 
 
-_NO_DROP = (0, 0, 1.0, 0, 0, None)  # on, threshold, scale, seed, host step, device step
+_NO_DROP = (0, 0, 1.0, 0, 0, 0)  # on, threshold, scale, seed, host step, device step's address
 
 
 def _bad(name, x):
@@ -67,42 +73,47 @@ def _bad(name, x):
 def _vec(t, C, dev, name):
     if t.dtype is not torch.float32:
         raise TypeError(f"block_norm: {name} must be float32, got {t.dtype}")
-    if t.dim() != 1 or t.shape[0] != C or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"block_norm: {name} must be a contiguous [{C}] vector on {dev}")
+    if t.dim() != 1 or t.numel() != C or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"block_norm: {name} must be a contiguous [{C}] vector on the device of x")
 
 
 def _norm_args(nm, C, dev, name):
     """(kind, gamma pointer, beta pointer, epsilon), checked."""
     if nm is None:
-        return 0, None, None, 0.0
-    kind = KINDS.get(nm.kind)
+        return 0, 0, 0, 0.0
+    kind, g, b, eps = nm
+    kind = KINDS.get(kind)
     if kind is None:
         raise ValueError(f"block_norm: {name} kind {nm.kind!r} (layer or rms)")
-    g, b, eps = nm.gamma, nm.beta, float(nm.eps)
     if not eps > 0.0:
         raise ValueError(f"block_norm: {name} needs an epsilon > 0, got {nm.eps}")
     if g is not None:
         _vec(g, C, dev, name + ".gamma")
         g = g.data_ptr()
+    else:
+        g = 0
     if b is not None:
         if kind == 2:
             raise ValueError(f"block_norm: {name}: an RMSNorm has no beta")
         _vec(b, C, dev, name + ".beta")
         b = b.data_ptr()
+    else:
+        b = 0
     return kind, g, b, eps
 
 
 def _common(x, gate, drop):
-    """(rows, columns, gate mode, rows per gate row, dropout arguments), checked."""
-    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float32:
-        raise TypeError(f"block_norm: expected bfloat16 or float32, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] < 1:
+    """(rows, columns, device index, gate mode, rows per gate row, dropout arguments), checked."""
+    dt, shape, dev = x.dtype, x.shape, x.get_device()
+    if dt is not torch.bfloat16 and dt is not torch.float32:
+        raise TypeError(f"block_norm: expected bfloat16 or float32, got {dt}")
+    if not shape or shape[-1] < 1:
         raise ValueError("block_norm: x needs at least one column")
     if not x.is_contiguous():
         raise ValueError("block_norm: x must be contiguous")
-    C, dev = x.shape[-1], x.device
+    C = shape[-1]
     M = x.numel() // C
-    if C > MAX_COLS and x.is_cuda:
+    if C > MAX_COLS and dev >= 0:
         raise ValueError(f"block_norm: rows of at most {MAX_COLS} columns, got {C}")
     mode, rpg = 0, 1
     if gate is not None:
@@ -110,43 +121,36 @@ def _common(x, gate, drop):
             _vec(gate, C, dev, "gate")
             mode, rpg = 1, M or 1
         else:
-            if gate.dim() != 2 or gate.shape[1] != C or gate.dtype is not x.dtype or gate.device != dev \
+            if gate.dim() != 2 or gate.shape[1] != C or gate.dtype is not dt or gate.get_device() != dev \
                     or not gate.is_contiguous():
-                raise ValueError(f"block_norm: gate must be fp32 [{C}] or {x.dtype} [groups, {C}], contiguous, on {dev}")
+                raise ValueError(f"block_norm: gate must be fp32 [{C}] or {dt} [groups, {C}], contiguous, on the device of x")
             G = gate.shape[0]
             if M and (G == 0 or M % G):
                 raise ValueError(f"block_norm: {M} rows do not divide into {G} gate groups")
             mode, rpg = 2, M // G if G else 1
     if drop is None:
-        return M, C, mode, rpg, _NO_DROP
+        return M, C, dev, mode, rpg, _NO_DROP
     thr, ds = DR.threshold(drop.rate)
-    host, step = DR.step_args(drop.step, dev)
-    return M, C, mode, rpg, (1, thr, ds, DR._signed(drop.seed), host, step)
+    host, step = DR.step_args(drop.step, x.device)
+    return M, C, dev, mode, rpg, (1, thr, ds, DR._signed(drop.seed), host, 0 if step is None else step.data_ptr())
 
 
-def _pointers(x, tensors, names):
-    """Data pointers of the tensors that must look like x (None where absent)."""
-    out, dt, shp, dev = [], x.dtype, x.shape, x.device
-    for t, name in zip(tensors, names):
-        if t is None:
-            out.append(None)
-            continue
-        if t.dtype is not dt or t.shape != shp or t.device != dev or not t.is_contiguous():
-            _bad(name, x)
-        out.append(t.data_ptr())
-    return out
+def _like(x, dt, dev, n, strides, t, name):
+    """Data pointer of a tensor that must look like x (0 where absent)."""
+    if t is None:
+        return 0
+    if t.dtype is not dt or t.get_device() != dev or t.numel() != n or not t.is_contiguous() \
+            or (t.stride() != strides and t.shape != x.shape):
+        _bad(name, x)  # contiguous, as many values, equal strides: the same rows
+    return t.data_ptr()
 
 
-def _apart(outs, ins, size):
-    """No output may overlap an input (pointer, name, whether the very same buffer will do) or another
-    output.  Every element is read before it is written, by the same thread."""
-    for k, (o, on) in enumerate(outs):
-        for i, iname, same in ins:
-            if -size < o - i < size and not (o == i and same):
-                raise ValueError(f"block_norm: {on} overlaps {iname}")
-        for p, pn in outs[:k]:
-            if -size < o - p < size:
-                raise ValueError(f"block_norm: {on} overlaps {pn}")
+def _apart(o, on, size, ins):
+    """Output ``o`` may not overlap an input (pointer, name, whether the very same buffer will do).  Every
+    element is read before it is written, by the same thread."""
+    for i, name, same in ins:
+        if -size < o - i < size and i and not (o == i and same):
+            raise ValueError(f"block_norm: {on} overlaps {name}")
 
 
 def _gate_apart(gate, outs, size):
@@ -157,39 +161,37 @@ def _gate_apart(gate, outs, size):
 
 
 def _stats_ok(stats, M, dev):
-    if stats.dtype is not torch.float32 or tuple(stats.shape) != (4, M) or stats.device != dev \
+    if stats.dtype is not torch.float32 or stats.shape != (4, M) or stats.get_device() != dev \
             or not stats.is_contiguous():
-        raise ValueError(f"block_norm: stats must be a contiguous fp32 [4, {M}] on {dev}")
+        raise ValueError(f"block_norm: stats must be a contiguous fp32 [4, {M}] on the device of x")
 
 
 def block_norm_fwd(x, *, res=None, post=None, gate=None, scale: float = 1.0, drop=None, pre=None, h=None, u=None,
                    stats=None):
     """Writes ``h`` (if given) and ``u`` (with ``pre``); ``stats`` (:func:`block_norm_stats`) for a
     backward pass.  Returns (h, u).  ``h`` may be ``res`` or ``x``; nothing else may overlap an input."""
-    M, C, mode, rpg, d = _common(x, gate, drop)
-    dev = x.device
+    M, C, dev, mode, rpg, d = _common(x, gate, drop)
     if (pre is None) != (u is None):
         raise ValueError("block_norm: u goes with pre")
     if h is None and u is None:
         raise ValueError("block_norm: nothing to write (h and u are None)")
     k1, g1, b1, e1 = _norm_args(post, C, dev, "post")
     k2, g2, b2, e2 = _norm_args(pre, C, dev, "pre")
-    xp = x.data_ptr()
-    rp, hp, up = _pointers(x, (res, h, u), ("res", "h", "u"))
+    dt, n, st, xp = x.dtype, M * C, x.stride(), x.data_ptr()
+    rp = _like(x, dt, dev, n, st, res, "res")
+    hp = _like(x, dt, dev, n, st, h, "h")
+    up = _like(x, dt, dev, n, st, u, "u")
     if stats is not None:
         _stats_ok(stats, M, dev)
-    f32 = x.dtype is torch.float32
-    size = M * C * (4 if f32 else 2)
-    ins = [(xp, "x", True)] if rp is None else [(xp, "x", True), (rp, "res", True)]
-    if up is not None:  # u is written after others have read, and h written before it
-        _apart([(up, "u")], [(i, n, False) for i, n, _ in ins], size)
-    outs = [] if hp is None else [(hp, "h")]
-    if up is not None and hp is not None:
-        outs.append((up, "u"))
-    _apart(outs, ins, size)
+    f32 = dt is torch.float32
+    size = n * (4 if f32 else 2)
+    if hp:
+        _apart(hp, "h", size, ((xp, "x", True), (rp, "res", True)))
+    if up:  # u is written after others have read, and h written before it
+        _apart(up, "u", size, ((xp, "x", False), (rp, "res", False), (hp, "h", False)))
     if mode == 2:
-        _gate_apart(gate, [(p, n) for p, n in ((hp, "h"), (up, "u")) if p is not None], size)
-    if not x.is_cuda:
+        _gate_apart(gate, [(p, n) for p, n in ((hp, "h"), (up, "u")) if p], size)
+    if dev < 0:
         hv, uv, st = _ref_fwd(x, res, post, gate, scale, drop, pre, M, C, rpg)
         if h is not None:
             h.copy_(hv.view(x.shape).to(h.dtype))
@@ -198,10 +200,11 @@ def block_norm_fwd(x, *, res=None, post=None, gate=None, scale: float = 1.0, dro
         if stats is not None:
             stats.copy_(st)
         return h, u
-    gp = None if gate is None else gate.data_ptr()
-    aligned = C % 8 == 0 and not (xp | (rp or 0) | (hp or 0) | (up or 0) | ((gp or 0) if mode == 2 else 0)) & 15
-    hip_on(dev, "ptg_block_norm_fwd", xp, rp, gp, hp, up, g1, b1, g2, b2, None if stats is None else stats.data_ptr(),
-           M, C, f32, aligned, k1, e1, k2, e2, mode, rpg, scale, d[0], d[1], d[2], d[3], d[4], ptr(d[5]))
+    gp = 0 if gate is None else gate.data_ptr()
+    aligned = C % 8 == 0 and not (xp | rp | hp | up | (gp if mode == 2 else 0)) & 15
+    hip_on(x.device, "ptg_block_norm_fwd",
+           _FWD.pack(xp, rp, gp, hp, up, g1, b1, g2, b2, 0 if stats is None else stats.data_ptr(), d[5], M, C, f32, aligned,
+                     k1, k2, mode, rpg, d[0], d[1], d[3], d[4], e1, e2, scale, d[2]))
     return h, u
 
 
@@ -212,8 +215,7 @@ def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1
     ``dpost`` / ``dpre`` = (dgamma, dbeta), fp32 [C] or None where the norm has none.  ``dx`` and ``dres``
     may each be one of x, res, du and dh; nothing else may overlap.  ``workspace``:
     :func:`block_norm_workspace` (None: allocated here)."""
-    M, C, mode, rpg, d = _common(x, gate, drop)
-    dev = x.device
+    M, C, dev, mode, rpg, d = _common(x, gate, drop)
     if (pre is None) != (du is None):
         raise ValueError("block_norm: du goes with pre")
     if pre is None and dh is None:
@@ -222,11 +224,15 @@ def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1
         raise ValueError("block_norm: no gradient is asked for")
     k1, g1, b1, _ = _norm_args(post, C, dev, "post")
     k2, g2, _, _ = _norm_args(pre, C, dev, "pre")
-    xp = x.data_ptr()
-    rp, up, hp, dxp, drp = _pointers(x, (res, du, dh, dx, dres), ("res", "du", "dh", "dx", "dres"))
+    dt, n, st, xp = x.dtype, M * C, x.stride(), x.data_ptr()
+    rp = _like(x, dt, dev, n, st, res, "res")
+    up = _like(x, dt, dev, n, st, du, "du")
+    hp = _like(x, dt, dev, n, st, dh, "dh")
+    dxp = _like(x, dt, dev, n, st, dx, "dx")
+    drp = _like(x, dt, dev, n, st, dres, "dres")
     _stats_ok(stats, M, dev)
     if dgate is not None and (gate is None or dgate.shape != gate.shape or dgate.dtype is not gate.dtype
-                              or dgate.device != dev or not dgate.is_contiguous()):
+                              or dgate.get_device() != dev or not dgate.is_contiguous()):
         raise ValueError("block_norm: dgate must match gate")
     vecs = []
     for g, nm, name in ((dpost, post, "dpost"), (dpre, pre, "dpre")):
@@ -239,40 +245,44 @@ def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1
                     raise ValueError(f"block_norm: {name} asks for the gradient of an absent {part}")
                 _vec(t, C, dev, name)
             vecs.append(t)
-    f32 = x.dtype is torch.float32
-    size = M * C * (4 if f32 else 2)
-    outs = [(p, n) for p, n in ((dxp, "dx"), (drp, "dres")) if p is not None]
-    _apart(outs, [(p, n, True) for p, n in ((xp, "x"), (rp, "res"), (up, "du"), (hp, "dh")) if p is not None], size)
+    f32 = dt is torch.float32
+    size = n * (4 if f32 else 2)
+    ins = ((xp, "x", True), (rp, "res", True), (up, "du", True), (hp, "dh", True))
+    outs = [(p, n) for p, n in ((dxp, "dx"), (drp, "dres")) if p]
+    for p, name in outs:
+        _apart(p, name, size, ins)
+    if dxp and drp:
+        _apart(drp, "dres", size, ((dxp, "dx", False),))
     if mode == 2:
         _gate_apart(gate, outs, size)
         if dgate is not None:
-            _gate_apart(dgate, outs + [(p, n) for p, n in ((xp, "x"), (rp, "res"), (up, "du"), (hp, "dh"))
-                                       if p is not None], size)
+            _gate_apart(dgate, outs + [(p, n) for p, n, _ in ins if p], size)
             _gate_apart(dgate, [(gate.data_ptr(), "gate")], gate.numel() * gate.element_size())
     if M == 0:
         for t in (dgate, *vecs):
             if t is not None:
                 t.zero_()
         return dx, dres
-    if not x.is_cuda:
+    if dev < 0:
         _ref_bwd(x, stats, res, post, gate, scale, drop, pre, du, dh, dx, dres, dgate, vecs, M, C, rpg)
         return dx, dres
     need = block_norm_workspace_floats(M, C, M // rpg if mode == 2 else 1)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.float32, device=dev)
-    elif workspace.dtype is not torch.float32 or workspace.device != dev or workspace.numel() < need \
+        workspace = torch.empty(need, dtype=torch.float32, device=x.device)
+    elif workspace.dtype is not torch.float32 or workspace.get_device() != dev or workspace.numel() < need \
             or not workspace.is_contiguous():
-        raise ValueError(f"block_norm: workspace must hold {need} contiguous floats on {dev}")
+        raise ValueError(f"block_norm: workspace must hold {need} contiguous floats on the device of x")
     if mode == 2 and dgate is None:
         dgate = torch.empty_like(gate)  # written all the same
-    gp = None if gate is None else gate.data_ptr()
-    dgp = None if dgate is None else dgate.data_ptr()
-    bits = xp | (rp or 0) | (up or 0) | (hp or 0) | (dxp or 0) | (drp or 0)
+    gp = 0 if gate is None else gate.data_ptr()
+    dgp = 0 if dgate is None else dgate.data_ptr()
+    bits = xp | rp | up | hp | dxp | drp
     if mode == 2:
         bits |= gp | dgp
-    hip_on(dev, "ptg_block_norm_bwd", xp, rp, gp, up, hp, dxp, drp, g1, b1, g2, stats.data_ptr(), ptr(vecs[0]),
-           ptr(vecs[1]), ptr(vecs[2]), ptr(vecs[3]), dgp, workspace.data_ptr(), M, C, f32, C % 8 == 0 and not bits & 15,
-           k1, k2, mode, rpg, scale, d[0], d[1], d[2], d[3], d[4], ptr(d[5]))
+    v = [0 if t is None else t.data_ptr() for t in vecs]
+    hip_on(x.device, "ptg_block_norm_bwd",
+           _BWD.pack(xp, rp, gp, up, hp, dxp, drp, g1, b1, g2, stats.data_ptr(), *v, dgp, workspace.data_ptr(), d[5], M, C, f32,
+                     C % 8 == 0 and not bits & 15, k1, k2, mode, rpg, d[0], d[1], d[3], d[4], scale, d[2]))
     return dx, dres
 
 

@@ -45,6 +45,14 @@ def test_gate_groups(hip_built, G, rpg, C):
     compare(t, both(t))
 
 
+@pytest.mark.parametrize("G,rpg", [(1, 29), (1, 62), (1, 200), (3, 70), (600, 62), (2, 8), (257, 5), (2000, 17)])
+@pytest.mark.parametrize("C", [7, 24, 48, 520])
+def test_gate_groups_shared_and_own(hip_built, G, rpg, C):
+    """Groups whose rows a workgroup's slots share, and groups that a slot goes through alone."""
+    t = make(G * rpg, C, "rms", "layer", G, True, torch.float32, "cuda")
+    compare(t, both(t, drop=DROP), drop=DROP)
+
+
 def test_unaligned_bases(hip_built):
     t = make(7, 64, "layer", "rms", 7, True, torch.bfloat16, "cuda")
 
