@@ -25,6 +25,7 @@ struct BlkArgs {
   DropArgs d;
   long M, rpg, items;  // rows per gate group; work items (see RowIter)
   int C, tpr, slotwise, sub, nvec;
+  int vecs;  // floats of the column vectors in LDS (wide rows: 0 where they are read from L2)
 };
 
 // Arguments of the C entries, one block of 64-bit fields (a call with as many arguments of its own costs the
@@ -277,10 +278,11 @@ struct Lane {
   }
 };
 
-// Column vectors (affine parameters, a gate row).  Rows of up to 2048 columns hold those that are there
-// in LDS (dynamic, [vector][2][C/2 rounded up]), as two planes of 4 values a thread so that a wave reads 16
-// bytes a lane without bank conflicts: in registers they would cost up to 40 of the 128 that leave four
-// waves a SIMD.  Wider rows (NT = 1024) read them from L2.
+// Column vectors (affine parameters, a gate row) are in LDS (dynamic, [vector][2][C/2 rounded up]), as two
+// planes of 4 values a thread so that a wave reads 16 bytes a lane without bank conflicts: in registers they
+// would cost up to 40 of the 128 that leave four waves a SIMD.  Rows of up to 2048 columns have a place for
+// every vector; wider ones (NT = 1024) only for those that are there, and if those do not fit they are
+// read from L2, a wait for each (3892 x 4520 pre-norm forward: 43.0 us from L2, 34.7 from LDS).
 struct ColVec {
   const float* src;  // null: dflt everywhere
   float dflt;
@@ -288,13 +290,18 @@ struct ColVec {
 };
 template <int NT, int N>
 struct ColVecs {
-  static constexpr bool LDS = NT <= 512;
+  static constexpr bool ALL = NT <= 512;
   ColVec v[N];
-  int half;
+  int half, place[N];
+  bool lds_on;
   // All vectors' loads are issued before the first store: one trip to memory, not one for each.
-  PTG_DEV void init(float* lds, int C, int tid) {
+  PTG_DEV void init(float* lds, int C, int tid, bool on) {
     half = ((C + 7) & ~7) >> 1;
-    if (!LDS) return;
+    lds_on = ALL || on;
+    int used = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) place[k] = ALL ? k : v[k].src ? used++ : 0;
+    if (!lds_on) return;
     for (int c = tid * 4; c < 2 * half; c += NT * 4) {
       float4 t[N];
 #pragma unroll
@@ -315,29 +322,41 @@ struct ColVecs {
         t[k].x *= v[k].mul; t[k].y *= v[k].mul; t[k].z *= v[k].mul; t[k].w *= v[k].mul;
       }
 #pragma unroll
-      for (int k = 0; k < N; ++k) *(float4*)(lds + 2 * k * half + ((c >> 2) & 1) * half + (c >> 3) * 4) = t[k];
+      for (int k = 0; k < N; ++k)
+        if (ALL || v[k].src) *(float4*)(lds + 2 * place[k] * half + ((c >> 2) & 1) * half + (c >> 3) * 4) = t[k];
     }
   }
   // c0 of a lane without columns: any that exist
   PTG_DEV void get(const float* lds, int k, float* f, int c0, int nv) const {
-    if (LDS) {
-      const float* p = lds + 2 * k * half + (c0 >> 1);
+    if (ALL || (lds_on && v[k].src)) {
+      const float* p = lds + 2 * place[k] * half + (c0 >> 1);
       const float4 a = *(const float4*)p, b = *(const float4*)(p + half);
       f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
       f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else if (!v[k].src) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = v[k].dflt * v[k].mul;
     } else {
-      if (v[k].src && nv == 8) {
+      if (nv == 8) {
         __builtin_memcpy(f, v[k].src + c0, 32);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = v[k].src && j < nv ? v[k].src[c0 + j] : v[k].dflt;
+        for (int j = 0; j < 8; ++j) f[j] = j < nv ? v[k].src[c0 + j] : v[k].dflt;
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] *= v[k].mul;
     }
   }
 };
-static inline int col_vec_bytes(int nt, int C, int n) { return nt <= 512 ? n * ((C + 7) & ~7) * 4 : 0; }
+constexpr int VECS_MOST = 128 * 1024;
+// bytes of the vectors of a workgroup of nt threads; 0: read from L2 (more than `most`, or none there)
+static inline int col_vec_bytes(int nt, int C, int n, const bool* there, int most) {
+  const int one = ((C + 7) & ~7) * 4;
+  if (nt <= 512) return n * one;
+  int bytes = 0;
+  for (int k = 0; k < n; ++k) bytes += there[k] ? one : 0;
+  return bytes <= most ? bytes : 0;
+}
 
 template <bool ALN>
 PTG_DEV void row_keep(const BlkArgs& a, uint64_t step, long at, uint32_t off, bool* k) {

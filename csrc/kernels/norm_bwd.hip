@@ -42,7 +42,7 @@ PTG_DEV void sum_cols(const float* lds, int tid, int tpr, int C, D* dst) {
     else dst[c] = s;
   }
 }
-// vectors joined at a time at the end: what LDS holds next to the column vectors
+// vectors joined at a time at the end; 16-wave workgroups join them in the place of the column vectors too
 template <int NT>
 constexpr int flush_vecs() { return NT <= 512 ? 5 : 3; }
 
@@ -98,8 +98,8 @@ __global__ __launch_bounds__(NT, 2) void block_norm_bwd_k(BlkArgs a) {
   cv.v[G2] = {PR ? a.g2 : nullptr, 1.f, 1.f};
   const float fs = DROP ? a.scale * a.d.scale : a.scale;  // scale and keep scale, times the gate: gt
   cv.v[GV] = {a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, 1.f, fs};
-  cv.init(vecs, C, tid);
-  float* cols = vecs + (cv.LDS ? 8 * cv.half : 0);
+  cv.init(vecs, C, tid, a.vecs);
+  float* cols = vecs + a.vecs;
   float ag1[8], ab1[8], ag2[8], ab2[8], agt[8], gt[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) { ag1[j] = 0.f; ab1[j] = 0.f; ag2[j] = 0.f; ab2[j] = 0.f; agt[j] = 0.f; gt[j] = fs; }
@@ -251,6 +251,7 @@ __global__ __launch_bounds__(NT, 2) void block_norm_bwd_k(BlkArgs a) {
     put_cols<LPR, NT>(acc, cols + v++ * col_floats<LPR, NT>(), tid, mul);
   };
   __syncthreads();
+  if (NT > 512) cols = vecs;  // no longer needed
   if (PR) {
     flush(ag2, 1.f);
     if (a.kind2 == NORM_LAYER) flush(ab2, 1.f);
@@ -343,10 +344,15 @@ void plan(BlkArgs& a, const Shape& s, int& grid) {
 template <typename T, int LPR, int NT, bool ALN, bool PO, bool PR, bool GG, bool DROP>
 void bwd_run(const BlkArgs& a, int grid, hipStream_t st) {
   auto kern = block_norm_bwd_k<T, LPR, NT, ALN, PO, PR, GG, DROP>;
-  const int lds = col_vec_bytes(NT, a.C, 4) + flush_vecs<NT>() * col_floats<LPR, NT>() * 4;
+  const bool there[4] = {PO && a.g1, PO && a.b1, PR && a.g2, a.gate_mode == GATE_VEC};
+  constexpr int one = col_floats<LPR, NT>() * 4;  // a vector's join
+  const int vb = col_vec_bytes(NT, a.C, 4, there, VECS_MOST - one), fb = flush_vecs<NT>() * one;
+  const int lds = NT <= 512 ? vb + fb : vb + one > fb ? vb + one : fb;
+  BlkArgs b = a;
+  b.vecs = vb / 4;
   static uint64_t set = 0;  // devices whose limit is raised
-  if (LPR == 64) ptg_allow_lds((const void*)kern, 128 * 1024, set);
-  kern<<<grid, NT, lds, st>>>(a);
+  if (LPR == 64) ptg_allow_lds((const void*)kern, VECS_MOST, set);
+  kern<<<grid, NT, lds, st>>>(b);
 }
 template <typename T, bool ALN, bool PO, bool PR, bool GG, bool DROP>
 void bwd_go(const BlkArgs& a, const Shape& s, int grid, hipStream_t st) {

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
   cv.v[B2] = {PR ? a.b2 : nullptr, 0.f, 1.f};
   const float sc = DROP ? a.scale * a.d.scale : a.scale;  // scale and keep scale, times the gate
   cv.v[GV] = {a.gate_mode == GATE_VEC ? (const float*)a.gate : nullptr, 1.f, sc};
-  cv.init(vecs, C, tid);
+  cv.init(vecs, C, tid, a.vecs);
   const float lay1 = a.kind1 == NORM_LAYER ? 1.f : 0.f, lay2 = a.kind2 == NORM_LAYER ? 1.f : 0.f;
   const bool full = C == tpr * 8;
   __syncthreads();
@@ -108,14 +108,20 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
 
 namespace {
 // Four waves a SIMD; three for rows above 1024 columns, which read more rows at a time as it is (32768 x 2048,
-// forward and backward together: 276 us with four, 259 with three; 401408 x 64: 56.9 with four, 58.2 with three).
+// forward and backward together: 276 us with four, 259 with three; 401408 x 64: 56.9 with four, 58.2 with three).  Above 2048 columns a workgroup is 16 waves, one a CU (4096 x 8192 forward:
+// 73.7 us; 76.6 with two a CU, 93.9 on three quarters of the CUs).
 template <typename T, bool ALN, bool PO, bool PR, bool DROP>
 int fwd_launch(const BlkArgs& a, hipStream_t stream) {
   auto go = [&](auto kern, int nt, int tpr) {
     BlkArgs b = a;
     b.tpr = tpr;
-    const long slots = nt / tpr, wgs = (a.M + slots - 1) / slots, cap = (a.C <= 1024 ? 1024L : 768L) * 256 / nt;
-    kern<<<(int)(wgs < cap ? wgs : cap), nt, col_vec_bytes(nt, a.C, 5), stream>>>(b);
+    const long slots = nt / tpr, wgs = (a.M + slots - 1) / slots, cap = a.C <= 1024 ? 1024 : a.C <= 2048 ? 768 : 256;
+    const bool there[5] = {a.kind1 && a.g1, a.kind1 && a.b1, a.kind2 && a.g2, a.kind2 && a.b2, a.gate_mode == GATE_VEC};
+    const int lds = col_vec_bytes(nt, a.C, 5, there, VECS_MOST);
+    b.vecs = lds / 4;
+    static uint64_t set = 0;  // devices whose limit is raised (only 16-wave workgroups get there)
+    if (lds > 64 * 1024) ptg_allow_lds((const void*)kern, VECS_MOST, set);
+    kern<<<(int)(wgs < cap ? wgs : cap), nt, lds, stream>>>(b);
   };
   const int C = a.C;
   if (C <= 16) go(block_norm_fwd_k<T, 2, 256, ALN, PO, PR, DROP>, 256, 2);
