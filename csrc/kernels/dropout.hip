@@ -107,10 +107,22 @@ __global__ void drop_advance_k(long* step) { *step += 1; }
 
 extern "C" {
 
-int ptg_dropout(const void* x, void* y, long n, int f32, int thr, float scale, long seed, long step,
-                const void* step_dev, long mid, long inner, hipStream_t stream) {
+// Arguments, 64 bits each (one block costs the host less than as many arguments)
+struct DropCall {
+  const void* x;
+  void* y;
+  const void* step_dev;
+  int64_t n, f32, thr, seed, step, mid, inner;
+  double scale;
+};
+int ptg_dropout(const void* call, hipStream_t stream) {
+  const DropCall& c = *(const DropCall*)call;
+  const void* x = c.x;
+  void* y = c.y;
+  const long n = c.n, mid = c.mid, inner = c.inner;
+  const bool f32 = c.f32;
   if (n <= 0) return 0;
-  const DropArgs d = drop_args(thr, scale, seed, step, step_dev);
+  const DropArgs d = drop_args((int)c.thr, (float)c.scale, c.seed, c.step, c.step_dev);
   const int vec = (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
   const long n8 = (n + 7) / 8;
   const int grid = (int)((n8 + 255) / 256 < 4096 ? (n8 + 255) / 256 : 4096);

@@ -13,6 +13,8 @@
 // The products run on 16 + u; acc starts from MFMAs with -(16 + z) in place of the weights, which leaves
 // sum (u - z) x.  Both products are exact in fp32, and the offset costs at most (16 + 15) / |u - z| of an
 // fp32 rounding.  Scales multiply the fp32 sum of a group, never a weight.
+#include <limits.h>
+
 #include "common.h"
 
 namespace {
@@ -471,17 +473,30 @@ int ptg_int4_ws(int M, int N, int K, int group, void* floats) {
   return 0;
 }
 
-// x: 16-byte aligned; w, scale, zero: tile layout; group 32, 64 or 128; zero null: 8 everywhere; act 0 linear, 1 ReLU
-int ptg_int4_dense(const void* x, const void* w, const void* scale, const void* zero, const void* bias, void* y,
-                   void* ws, int M, int N, int K, int group, int act, int f32, hipStream_t stream) {
-  if (M <= 0 || N <= 0) return 0;
+// Arguments, 64 bits each.  x: 16-byte aligned; w, scale, zero: tile layout; group 32, 64 or 128; zero null: 8
+// everywhere; act 0 linear, 1 ReLU
+struct Int4Call {
+  const bf16_t* x;
+  const uint8_t* w;
+  const bf16_t* scale;
+  const uint8_t* zero;
+  const float* bias;
+  void* y;
+  float* ws;
+  int64_t M, N, K, group, act, f32;
+};
+int ptg_int4_dense(const void* call, hipStream_t stream) {
+  const Int4Call& c = *(const Int4Call*)call;
+  if (c.M <= 0 || c.N <= 0) return 0;
+  if (c.M > INT_MAX || c.N > INT_MAX || c.K > INT_MAX) return (int)hipErrorInvalidValue;
+  const int M = (int)c.M, N = (int)c.N, K = (int)c.K, group = (int)c.group;
   // a block of rows or of outputs stays below 2 GiB
-  if ((group != 32 && group != 64 && group != 128) || K < group || K % group || K > (1 << 22) || ((uintptr_t)x & 15))
+  if ((group != 32 && group != 64 && group != 128) || K < group || K % group || K > (1 << 22) || ((uintptr_t)c.x & 15))
     return (int)hipErrorInvalidValue;
   const Plan4 p = plan4(M, N, K, group);
-  if (p.splits > 1 && !ws) return (int)hipErrorInvalidValue;
-  const Args4 a{(const bf16_t*)x, (const uint8_t*)w, (const bf16_t*)scale, (const uint8_t*)zero, (const float*)bias,
-                y, p.splits > 1 ? (float*)ws : nullptr, M, N, K, (K + QT_K - 1) / QT_K, act, f32};
+  if (p.splits > 1 && !c.ws) return (int)hipErrorInvalidValue;
+  const Args4 a{c.x, c.w, c.scale, c.zero, c.bias, c.y, p.splits > 1 ? c.ws : nullptr, M, N, K, (K + QT_K - 1) / QT_K,
+                (int)c.act, (int)c.f32};
   if (group == 32) return go4g<1>(p, a, stream);
   if (group == 64) return go4g<2>(p, a, stream);
   return go4g<4>(p, a, stream);

@@ -16,6 +16,7 @@ tensors the reference below.
 from __future__ import annotations
 
 import math
+import struct
 from typing import NamedTuple
 
 import torch
@@ -23,6 +24,7 @@ import torch
 from ._util import hip_on, on_device, ptr
 
 _M64 = (1 << 64) - 1
+_CALL = struct.Struct("=3Q7qd")  # DropCall of dropout.hip
 
 
 class Drop(NamedTuple):
@@ -68,20 +70,31 @@ def mix_seed(seed: int, stream: int) -> int:
 
 def noise_dims(shape, noise_shape) -> tuple[int, int, int]:
     """(outer, mid, inner) of ``shape`` whose mask is shared over mid."""
-    shape = tuple(int(s) for s in shape)
-    n = math.prod(shape)
     if noise_shape is None:
-        return n, 1, 1
-    noise = tuple(s if v is None else int(v) for v, s in zip(noise_shape, shape))
-    if len(noise_shape) != len(shape) or any(v not in (1, s) for v, s in zip(noise, shape)):
-        raise ValueError(f"dropout: noise_shape {tuple(noise_shape)} does not broadcast to {shape}")
-    shared = [k for k, (v, s) in enumerate(zip(noise, shape)) if v == 1 and s > 1]
-    if not shared:
-        return n, 1, 1
-    lo, hi = shared[0], shared[-1] + 1
-    if any(noise[k] != 1 for k in range(lo, hi)):
-        raise NotImplementedError(f"dropout: noise_shape {noise} shares two separate runs of axes of {shape}")
-    return math.prod(shape[:lo]), math.prod(shape[lo:hi]), math.prod(shape[hi:])
+        return math.prod(shape), 1, 1
+    outer, mid, inner = 1, 1, 1
+    run = 0  # 0 before, 1 in, 2 behind the shared axes
+    again = False
+    if len(noise_shape) != len(shape):
+        raise ValueError(f"dropout: noise_shape {tuple(noise_shape)} does not broadcast to {tuple(shape)}")
+    for s, v in zip(shape, noise_shape):
+        if v is None or v == s:
+            if run == 1 and s != 1:
+                run = 2
+            if run == 0:
+                outer *= s
+            else:
+                inner *= s
+        elif v == 1:
+            again = again or run == 2
+            run = 1
+            mid *= s
+        else:
+            raise ValueError(f"dropout: noise_shape {tuple(noise_shape)} does not broadcast to {tuple(shape)}")
+    if again:
+        raise NotImplementedError(f"dropout: noise_shape {tuple(noise_shape)} shares two separate runs of axes of "
+                                  f"{tuple(shape)}")
+    return (outer, mid, inner) if mid > 1 else (outer * mid * inner, 1, 1)
 
 
 def _pieces(blocks, step: int, seed: int):
@@ -129,7 +142,8 @@ def _run(name, x, rate, seed, step, out, noise_shape):
     xp, op, n, f32 = x.data_ptr(), out.data_ptr(), x.numel(), dt is torch.float32
     if xp != op and abs(xp - op) < n * (4 if f32 else 2):
         raise ValueError(f"{name}: input and output overlap")
-    hip_on(x.device, "ptg_dropout", xp, op, n, f32, thr, scale, _signed(seed), host, ptr(dev), mid, inner)
+    hip_on(x.device, "ptg_dropout",
+           _CALL.pack(xp, op, 0 if dev is None else dev.data_ptr(), n, f32, thr, _signed(seed), host, mid, inner, scale))
     return out
 
 

@@ -10,13 +10,15 @@ the kernel, CPU tensors the fp32 reference.  Inference only: codes have no gradi
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
 
-from ._util import hip_on, ptr
+from ._util import hip_on
 
 GROUPS = (32, 64, 128)
+_CALL = struct.Struct("=7Q6q")  # Int4Call of quant.hip
 ACT = {None: 0, "linear": 0, "relu": 1}
 
 
@@ -111,9 +113,11 @@ def int4_layout(codes, scale, zero=None, group: int = 128) -> Int4Weight:
     def group_rows(t):
         if t is None:
             return None
-        p = torch.zeros((Np, Kp // group), dtype=t.dtype, device=t.device)
-        p[:N, : K // group] = t
-        return p.view(Np // 16, 16, Kp // 128, 128 // group).permute(0, 2, 1, 3).contiguous()
+        p = t.contiguous()
+        if (Np, Kp) != (N, K):
+            p = torch.zeros((Np, Kp // group), dtype=t.dtype, device=t.device)
+            p[:N, : K // group] = t
+        return p.view(Np // 16, 16, Kp // 128, 128 // group).permute(0, 2, 1, 3).clone(memory_format=torch.contiguous_format)
 
     return Int4Weight(tiles, group_rows(scale), group_rows(zero), N, K, group)
 
@@ -209,7 +213,7 @@ def int4_dense_fwd(x, w: Int4Weight, bias, act, out, workspace=None):
         x = x.clone()  # the kernel reads 16 bytes at a time
         xp = x.data_ptr()
     need = int4_workspace_floats(B, w)
-    wp = None
+    wp = 0
     if need:
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.float32, device=dev)
@@ -217,6 +221,7 @@ def int4_dense_fwd(x, w: Int4Weight, bias, act, out, workspace=None):
                 or not workspace.is_contiguous():
             raise ValueError(f"int4_dense: workspace must hold {need} contiguous floats on {dev}")
         wp = workspace.data_ptr()
-    hip_on(dev, "ptg_int4_dense", xp, tiles.data_ptr(), w.scale.data_ptr(), ptr(w.zero),
-           None if bias is None else bias.data_ptr(), op, wp, B, n, k, w.group, relu, f32)
+    hip_on(dev, "ptg_int4_dense",
+           _CALL.pack(xp, tiles.data_ptr(), w.scale.data_ptr(), 0 if w.zero is None else w.zero.data_ptr(),
+                      0 if bias is None else bias.data_ptr(), op, wp, B, n, k, w.group, relu, f32))
     return out
