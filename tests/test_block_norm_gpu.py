@@ -53,6 +53,22 @@ def test_gate_groups_shared_and_own(hip_built, G, rpg, C):
     compare(t, both(t, drop=DROP), drop=DROP)
 
 
+@pytest.mark.parametrize("G,rpg", [(1, 40), (6, 3), (300, 1), (2, 301)])
+@pytest.mark.parametrize("C", [2056, 4101, 8192])
+@pytest.mark.parametrize("post", [None, "layer"])
+def test_gate_groups_wide(hip_built, G, rpg, C, post):
+    """Rows of 16 waves: a layer pair and grouped gates of 8192 columns just fit their vectors in LDS."""
+    t = make(G * rpg, C, post, "layer", G, True, torch.bfloat16, "cuda")
+    compare(t, both(t, drop=DROP), drop=DROP)
+
+
+@pytest.mark.parametrize("C", [3000, 6144, 8192])
+@pytest.mark.parametrize("post,pre", [("layer", "layer"), ("rms", "layer"), (None, "rms"), ("layer", None), (None, None)])
+def test_wide_vectors_in_and_out_of_lds(hip_built, C, post, pre):
+    t = make(530, C, post, pre, 0, True, torch.float32, "cuda")
+    compare(t, both(t, drop=DROP), drop=DROP)
+
+
 def test_unaligned_bases(hip_built):
     t = make(7, 64, "layer", "rms", 7, True, torch.bfloat16, "cuda")
 

@@ -85,3 +85,32 @@ def test_rate_statistics():
     assert abs(k - 0.75 * n) < 6 * (n * 0.75 * 0.25) ** 0.5
     a, b = D.keep_mask((n,), 0.5, 77, 3), D.keep_mask((n,), 0.5, 77, 4)
     assert abs(int((a == b).sum()) - n / 2) < 6 * (n / 4) ** 0.5
+
+
+def test_noise_dims_against_the_definition():
+    """Every shape of 1 and 3 with three axes and every noise shape of None, 1 and 3: the mask entries
+    that (outer, mid, inner) names are those of broadcasting, or the shape is refused."""
+    import itertools
+
+    for shape in itertools.product((1, 3), repeat=3):
+        for noise in itertools.product((None, 1, 3), repeat=3):
+            full = tuple(s if v is None else v for s, v in zip(shape, noise))
+            if any(v not in (1, s) for v, s in zip(full, shape)):
+                with pytest.raises(ValueError):
+                    D.noise_dims(shape, noise)
+                continue
+            shared = [k for k in range(3) if full[k] == 1 and shape[k] == 3]
+            if shared and any(full[k] == 3 for k in range(shared[0], shared[-1] + 1)):
+                with pytest.raises(NotImplementedError):
+                    D.noise_dims(shape, noise)
+                continue
+            outer, mid, inner = D.noise_dims(shape, noise)
+            n = full[0] * full[1] * full[2]
+            assert outer * mid * inner == shape[0] * shape[1] * shape[2]
+            want = torch.arange(n).view(full).expand(shape).reshape(-1)
+            if mid == 1:
+                assert torch.equal(want, torch.arange(len(want)))
+            else:
+                got = torch.arange(outer * inner).view(outer, 1, inner).expand(outer, mid, inner).reshape(-1)
+                assert torch.equal(got, want)
+    assert D.noise_dims((4, 5), None) == (20, 1, 1) and D.noise_dims((0, 5), (1, None)) == (0, 1, 1)
