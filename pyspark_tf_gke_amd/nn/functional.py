@@ -320,23 +320,31 @@ def _lower(nodes: list, input_idx: int) -> list:
         ops.append(G.Adapter(inner(layer), [src(ins[0])], k))
     NO.bind_drop_state(ops)
     _bn_bwd_links(ops)
-    # dense relu-mask hand-off as in the Sequential engine
+    # dense relu-mask hand-off as in the Sequential engine, where b is all that reads a's output: what another
+    # reader gives back is not masked
+    uses = _uses(ops)
     for a, b in zip(ops, ops[1:]):
         ia, ib = getattr(a, "inner", None), getattr(b, "inner", None)
         if isinstance(ia, E.DenseOp) and isinstance(ib, E.DenseOp) and not ib.big and ia.act == "relu" \
-                and b.inputs == [a.output]:
+                and b.inputs == [a.output] and len(uses[a.output]) == 1:
             ib.mask_for_prev, ib._prev_big, ib._prev_op = True, ia.big, ia
             ia.grad_masked_by_next = True
     return ops
 
 
-def _bn_bwd_links(ops) -> None:
-    """Conv -> BN -> ReLU (no residual) feeding exactly one ConvBNOp: that consumer's dgrad epilogue
-    computes the producer's BN backward sums (graph_ops.BN_BWD_EPI)."""
+def _uses(ops) -> dict:
+    """tensor -> the ops that read it, once for every input that it is"""
     uses: dict = {}
     for op in ops:
         for i in op.inputs:
             uses.setdefault(i, []).append(op)
+    return uses
+
+
+def _bn_bwd_links(ops) -> None:
+    """Conv -> BN -> ReLU (no residual) feeding exactly one ConvBNOp: that consumer's dgrad epilogue
+    computes the producer's BN backward sums (graph_ops.BN_BWD_EPI)."""
+    uses = _uses(ops)
     for a in ops:
         pa = getattr(a, "op", None)
         if not isinstance(pa, G.ConvBNOp) or not pa.relu or pa.residual:
