@@ -119,6 +119,28 @@ def _bf16(x, ws, key):
     return out
 
 
+def _own_channels(dx, C, ws, key):
+    """The gradient of the C channels that a convolution's input has, without the zero channels it was padded
+    to: whoever made that input knows nothing of them."""
+    if dx.shape[-1] == C:
+        return dx
+    out = ws.get(key, (*dx.shape[:-1], C), dx.dtype, dx.device)
+    out.copy_(dx[..., :C])
+    return out
+
+
+def _dgrad_sizes(w, x, ws, key):
+    """(filter, gradient buffer) of a data gradient like ``x``: the kernels take 8 input channels at a time, so a
+    filter of 4 gets 4 zero channels behind it."""
+    C = w.shape[-1]
+    if not x.is_cuda or C % 8 == 0:
+        return w, ws.get(key + "/dx", x.shape, torch.bfloat16, x.device)
+    Cw = -(-C // 8) * 8
+    ww = ws.get(key + "/wwide", (*w.shape[:-1], Cw), w.dtype, w.device, zero=True)
+    ww[..., :C] = w
+    return ww, ws.get(key + "/dxwide", (*x.shape[:-1], Cw), torch.bfloat16, x.device)
+
+
 class ConvOp(Op):
     def __init__(self, conv: L.Conv2D, prelu: L.PReLU | None, pool: L.MaxPooling2D | None):
         super().__init__()
@@ -321,7 +343,7 @@ class ConvOp(Op):
         dx = ws.get(self.name + "/dx", x.shape, torch.bfloat16, dev)
         K.conv2d_dgrad_halo_sparse(dzs, arg, self.conv.kernel.bf16, self.pad, dx, self._wflip_buf(ws, dev),
                                    flipped=getattr(self, "_wf_ready", False))
-        return dx
+        return _own_channels(dx, self.conv.cin, ws, self.name + "/dxc")
 
     def _backward_fused1(self, x, dy, ws, dev):
         """First layer, conv1.hip: one kernel from the pooled gradient to dW / dalpha / dbias."""
@@ -407,14 +429,15 @@ class ConvOp(Op):
     def _dgrad(self, x, dz, ws, dev, halo_dgrad):
         if self.stride != 1:
             raise NotImplementedError("dgrad for strided convolutions")
-        dx = ws.get(self.name + "/dx", x.shape, torch.bfloat16, dev)
         if halo_dgrad:
+            dx = ws.get(self.name + "/dx", x.shape, torch.bfloat16, dev)
             wf = self._wflip_buf(ws, dev)
             K.conv2d_dgrad_halo(dz, self.conv.kernel.bf16, self.pad, dx, wf,
                                 flipped=getattr(self, "_wf_ready", False))
         else:
-            K.conv2d_dgrad(dz, self.conv.kernel.bf16, self.pad, dx)
-        return dx
+            w, dx = _dgrad_sizes(self.conv.kernel.bf16, x, ws, self.name)
+            K.conv2d_dgrad(dz, w, self.pad, dx)
+        return _own_channels(dx, self.conv.cin, ws, self.name + "/dxc")
 
 
 class DenseOp(Op):

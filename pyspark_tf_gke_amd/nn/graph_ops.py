@@ -298,7 +298,8 @@ class ConvBNOp:
         dx = None
         if not self.first:
             ex = existing[0]
-            if ex is not None and ex.dtype == x.dtype and tuple(ex.shape) == tuple(x.shape):
+            if ex is not None and ex.dtype == x.dtype and tuple(ex.shape) == tuple(x.shape) \
+                    and (x.shape[-1] % 8 == 0 or not x.is_cuda):
                 conv_dgrad(dz, self.conv.kernel.bf16, self.stride, self.pad, ex, True, ws, self.name)
                 dx = ex
             else:
@@ -311,7 +312,9 @@ class ConvBNOp:
                     if K.conv_dgrad_bnstats(dz, self.conv.kernel.bf16, self.pad, dx, part, p._z, scale, shift):
                         p._bwd_stats_done = True
                         return [dx] + ([dres] if self.residual else [])
-                conv_dgrad(dz, self.conv.kernel.bf16, self.stride, self.pad, dx, False, ws, self.name)
+                w, dx = E._dgrad_sizes(self.conv.kernel.bf16, x, ws, self.name)
+                conv_dgrad(dz, w, self.stride, self.pad, dx, False, ws, self.name)
+                dx = E._own_channels(dx, self.conv.cin, ws, self.name + "/dxc")
         return [dx] + ([dres] if self.residual else [])
 
 
