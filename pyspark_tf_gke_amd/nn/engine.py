@@ -724,9 +724,14 @@ def lower(layers: list) -> list:
             raise NotImplementedError(type(l).__name__)
     if ops:
         ops[0].first = True
-    if any(isinstance(l, L.Dropout) for l in seq):
+    if any(isinstance(l, (L.Rescaling, L.Dropout)) for l in seq):
         from . import norm_ops as NO
 
+        # no gradient goes to weights in front of the first convolution either
+        for a, b in zip(ops, ops[1:]):
+            if not NO.bare(a) or not (NO.bare(b) or isinstance(b, ConvOp)):
+                break
+            b.first = True
         NO.bind_drop_state(ops)
     for k in range(1, len(ops)):
         ops[k].below = ops[k - 1]

@@ -80,8 +80,12 @@ class GraphPlan:
         self.input_idx = input_idx
         self.output_idx = output_idx
         self.ops = _lower(nodes, input_idx)
+        free = {input_idx}  # tensors with no weights behind them
         for op in self.ops:
-            op.first = all(i == input_idx for i in op.inputs)
+            conv = isinstance(getattr(op, "inner", getattr(op, "op", op)), (E.ConvOp, G.ConvBNOp))
+            op.first = all(i in (free if conv or NO.bare(op) else (input_idx,)) for i in op.inputs)
+            if op.first and NO.bare(op):
+                free.update(getattr(op, "outputs", (op.output,)))
 
     def forward(self, x, ws, training, pre_op=None):
         vals = {self.input_idx: x}

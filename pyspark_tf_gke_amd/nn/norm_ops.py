@@ -197,6 +197,9 @@ class BlockOp:
 
     def backward(self, gs, ws, existing=None):
         x, st, kw = self._x, self._st, self._kw
+        n_in = 1 + self.gate_input + self.res
+        if self.first and not self.params:
+            return [None] * n_in
         gs = list(gs)
         dh = gs.pop(0) if self.want_h else None
         du = gs.pop(0) if self.pre is not None else None
@@ -206,9 +209,6 @@ class BlockOp:
             du = ws.get(self.name + "/du0", x.shape, dt, dev)  # the normalised output led nowhere
             du.zero_()
         du = None if du is None else _float(du, ws, self.name + "/du16", dt).reshape(x.shape)
-        n_in = 1 + self.gate_input + self.res
-        if self.first and not self.params:
-            return [None] * n_in
         dx = None if self.first else ws.get(self.name + "/dx", x.shape, dt, dev)
         dres = ws.get(self.name + "/dres", x.shape, dt, dev) if self.res and not self.first else None
         dgate = None
@@ -272,6 +272,13 @@ class BlockNode:
 
     def _prep_input(self, x, ws):
         return self.op._prep_input(x, ws)
+
+
+def bare(op) -> bool:
+    """A Dropout, Rescaling or Multiply op (no weights): what reads the model's input through it alone is as good
+    as first."""
+    op = getattr(op, "inner", getattr(op, "op", op))
+    return isinstance(op, (DropoutOp, SeqBlockOp, BlockOp)) and not op.params
 
 
 def is_norm(layer) -> bool:

@@ -65,6 +65,25 @@ def test_layers_between_convolutions(fp32_host, filters):  # noqa: F811
     agree(compiled(nn.Model(inp, nn.Dense(2, name="head")(y))), *images(5, (8, 6, 3)), 1, 2e-5)
 
 
+@pytest.mark.parametrize("functional", [False, True])
+def test_rescaled_images_into_a_strided_convolution(functional):
+    """No gradient is wanted in front of the first weights: a strided convolution has none to give."""
+    L.reset_name_counters()
+    ls = [nn.Rescaling(1 / 255, name="f"), nn.Dropout(0.1, name="d"),
+          nn.Conv2D(16, 3, strides=2, padding="same", name="c"), nn.GlobalAveragePooling2D(name="p"),
+          nn.Dense(2, name="head")]
+    if functional:
+        inp = t = nn.Input(shape=(8, 6, 3))
+        for l in ls:
+            t = l(t)
+        m = compiled(nn.Model(inp, t))
+    else:
+        m = compiled(nn.Sequential([nn.Input(shape=(8, 6, 3)), *ls]))
+    x = np.random.default_rng(0).integers(0, 256, (5, 8, 6, 3), dtype=np.uint8)
+    out, g = engine_grads(m, x, np.ones((5, 2), np.float32))
+    assert all(bool(torch.isfinite(v).all()) and bool(v.any()) for v in g.values())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("front", sorted(FRONT))
 @pytest.mark.parametrize("channels", [3, 4])
