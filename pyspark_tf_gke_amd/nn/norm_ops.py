@@ -107,17 +107,17 @@ class DropoutOp(E.Op):
             return x
         x = _float(x, ws, self.name + "/x16")
         y = ws.get(self.name + "/y", x.shape, x.dtype, x.device)
-        return DR.dropout_fwd(x, self._d.rate, self._d.seed, self._d.step, y, self._noise(x))
-
-    def _noise(self, x):
-        return self.drop.noise_shape
+        self._shape = x.shape  # the mask goes by it
+        return DR.dropout_fwd(x, self._d.rate, self._d.seed, self._d.step, y, self.drop.noise_shape)
 
     def backward(self, dy, ws):
         if self._d is None or self.first:
             return dy
-        dy = _float(dy, ws, self.name + "/dy16")
+        if dy.numel() != self._shape.numel():
+            raise ValueError(f"{self.name}: a gradient of shape {tuple(dy.shape)} for an output of {tuple(self._shape)}")
+        dy = _float(dy, ws, self.name + "/dy16").reshape(self._shape)
         dx = ws.get(self.name + "/dx", dy.shape, dy.dtype, dy.device)
-        return DR.dropout_bwd(dy, self._d.rate, self._d.seed, self._d.step, dx, self._noise(dy))
+        return DR.dropout_bwd(dy, self._d.rate, self._d.seed, self._d.step, dx, self.drop.noise_shape)
 
 
 class BlockOp:
