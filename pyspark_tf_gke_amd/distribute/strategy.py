@@ -433,9 +433,20 @@ class MultiWorkerMirroredStrategy(Strategy):
                     break
                 self._rs(model, plan, b)
             return
-        hi = max(p.offset + p.numel for p in op.params)
+        hi = min(max(p.offset + p.numel for p in op.params), self._ready_below(model, op))
         if hi - self._launched >= self.bucket_elems:
             self._launch(model, hi)
+
+    def _ready_below(self, model, op) -> int:
+        """Where the gradients begin that ops in front of ``op`` have yet to write: a block boundary holds
+        parameters from both sides of a gate that is computed in between."""
+        if getattr(self, "_ready_ops", None) is not model.ops:
+            below, self._ready = model.store.total, {}
+            for o in model.ops:
+                self._ready[id(o)] = below
+                below = min([below, *(p.offset for p in o.params)])
+            self._ready_ops = model.ops
+        return self._ready[id(op)]
 
     def finish_gradients(self, model) -> None:
         if (self.dp_degree == 1 and not self.sharded_update) or self.in_round():
