@@ -7,7 +7,8 @@
 
 Both land next to this file so they travel with a ``gpurun`` snapshot and are what the Python
 process dlopens (no site-packages install, no JIT cache). Objects are rebuilt only when a source
-or header is newer than the object.
+or header is newer than the object, or when they were compiled with other flags: a HIP library carries the
+key of its flags, and so does the folder of its objects.
 
 Usage: ``python -m pyspark_tf_gke_amd._native.build [--force] [-j N]``
 """
@@ -15,6 +16,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import hashlib
 import os
 import shutil
 import subprocess
@@ -52,6 +54,19 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError(f"command failed ({r.returncode}): {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
 
 
+def _key(cmd: list[str]) -> str:
+    """Names the flags ``cmd`` in what they made."""
+    return "ptg_build_key=" + hashlib.sha256("\0".join(cmd).encode()).hexdigest()[:32]
+
+
+def _key_object(bdir: Path, key: str) -> Path:
+    src, obj = bdir / "build_key.cpp", bdir / "build_key.o"
+    src.write_text(f'extern "C" __attribute__((used)) const char ptg_build_key[] = "{key}";\n'
+                   'extern "C" const char* ptg_build_key_text() { return ptg_build_key; }\n')
+    _run([shutil.which("g++") or "g++", "-O1", "-fPIC", "-c", str(src), "-o", str(obj)])
+    return obj
+
+
 def build_hip(force: bool = False, jobs: int = 8, verbose: bool = True, checked: bool = False,
               variant: str | None = None, defines: tuple = ()) -> Path:
     """``checked``: the bounds-checked variant - every PTG_CHECKED_IDX site verifies its
@@ -67,11 +82,18 @@ def build_hip(force: bool = False, jobs: int = 8, verbose: bool = True, checked:
     # no packed fp32 arithmetic: the compiler forms v_pk_add/mul/fma_f32 from ordinary float code, and
     # some of their forms have given wrong results on this hardware
     flags = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-munsafe-fp-atomics",
-             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-result", "-I", str(CSRC / "kernels")] + (["-DPTG_CHECKED"] if checked else [])
-    flags += [f"-D{d}" for d in defines]
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-result"]
+    flags += (["-DPTG_CHECKED"] if checked else []) + [f"-D{d}" for d in defines]
+    key = _key(flags)  # not by paths: a tree may be copied after its build
+    flags += ["-I", str(CSRC / "kernels")]
     if not force and out_lib.exists() and srcs and \
-            out_lib.stat().st_mtime >= max(_newest_dep(s, headers) for s in srcs):
+            out_lib.stat().st_mtime >= max(_newest_dep(s, headers) for s in srcs) and \
+            key.encode() in out_lib.read_bytes():
         return out_lib  # up to date (objects need not exist: a snapshot ships only the library)
+    key_file = bdir / "build_key"
+    if not key_file.exists() or key_file.read_text() != key:
+        force = True  # objects of other flags, or of flags that nobody wrote down
+        key_file.unlink(missing_ok=True)
     objs, todo = [], []
     for s in srcs:
         o = bdir / (s.stem + ".o")
@@ -88,12 +110,13 @@ def build_hip(force: bool = False, jobs: int = 8, verbose: bool = True, checked:
 
     with cf.ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
         list(ex.map(compile_one, todo))
-    if force or todo or not out_lib.exists() or any(out_lib.stat().st_mtime < o.stat().st_mtime for o in objs):
-        tmp = out_lib.with_suffix(".so.tmp")
-        _run([hipcc, "--offload-arch=" + ARCH, "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)])
-        os.replace(tmp, out_lib)
-        if verbose:
-            print(f"[build] linked {out_lib}", flush=True)
+    key_file.write_text(key)
+    tmp = out_lib.with_suffix(".so.tmp")
+    _run([hipcc, "--offload-arch=" + ARCH, "-shared", "-fPIC", *map(str, objs), str(_key_object(bdir, key)), "-o",
+          str(tmp)])
+    os.replace(tmp, out_lib)
+    if verbose:
+        print(f"[build] linked {out_lib}", flush=True)
     return out_lib
 
 
