@@ -26,6 +26,7 @@ struct BlkArgs {
   long M, rpg, items;  // rows per gate group; work items (see RowIter)
   int C, tpr, slotwise, sub, nvec;
   int vecs;  // floats of the column vectors in LDS (wide rows: 0 where they are read from L2)
+  int over;  // an output lies on an input and rows are unaligned: see meet()
 };
 
 // Arguments of the C entries, one block of 64-bit fields (a call with as many arguments of its own costs the
@@ -53,6 +54,15 @@ struct BwdCall {
 static_assert(sizeof(FwdCall) == 27 * 8 && sizeof(BwdCall) == 32 * 8, "64-bit fields");
 
 typedef __attribute__((ext_vector_type(4))) unsigned int vu4_t;
+
+// The last group of an unaligned row reads columns of the lane before it as well (Lane::load).  Those may belong to
+// another wave, which must not write an output on top of them before they are read: where an output lies on an
+// input the waves of a workgroup meet once a row, between its loads and its first store.  A kernel whose row sums
+// come before that store (`summed`) has met there.
+template <int LPR, bool ALN>
+PTG_DEV void meet(const BlkArgs& a, bool summed) {
+  if (LPR == 64 && !ALN && !summed && a.over) __syncthreads();
+}
 
 // ---- sums over the LPR lanes of a row (every lane gets the sum) --------------------------------
 template <int CTRL>

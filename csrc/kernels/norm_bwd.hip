@@ -168,6 +168,7 @@ __global__ __launch_bounds__(NT, 2) void block_norm_bwd_k(BlkArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) gh[j] = fmaf(s2, gu[j] - fmaf(r[j], k2, k1), gh[j]);
     }
+    meet<LPR, ALN>(a, PR);
     if (a.dres) {
       t.set(gh);
       ln.store(t, a.dres, at, crows, C, con);
@@ -423,6 +424,8 @@ int ptg_block_norm_bwd(const void* call, hipStream_t stream) {
   a.gate_mode = gate_mode; a.rpg = gate_mode == GATE_GROUP ? rpg : 1; a.scale = (float)c.scale; a.drop = (int)c.drop;
   a.d = drop_args((int)c.thr, (float)c.dscale, c.seed, c.step, c.step_dev);
   a.dgate = dgate;
+  auto over = [&](const void* o) { return o && (o == c.x || o == c.res || o == c.du || o == c.dh); };
+  a.over = !aligned && (over(c.dx) || over(c.dres));
   const Shape s = shape_of(C);
   int grid;
   plan(a, s, grid);

@@ -84,6 +84,7 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = j < nv ? f[j] : 0.f;
     }
+    meet<LPR, ALN>(a, PO);
     if (a.h) {
       t.set(f);
       ln.store(t, a.h, at, crows, C, con);
@@ -158,6 +159,7 @@ int ptg_block_norm_fwd(const void* call, hipStream_t stream) {
   a.eps1 = (float)c.eps1; a.eps2 = (float)c.eps2;
   a.gate_mode = (int)c.gate_mode; a.rpg = c.rpg > 0 ? c.rpg : 1; a.scale = (float)c.scale; a.drop = (int)c.drop;
   a.d = drop_args((int)c.thr, (float)c.dscale, c.seed, c.step, c.step_dev);
+  a.over = !c.aligned && c.h && (c.h == c.x || c.h == c.res);
   if (c.f32) return c.aligned ? fwd_drop<float, true>(a, stream) : fwd_drop<float, false>(a, stream);
   return c.aligned ? fwd_drop<bf16_t, true>(a, stream) : fwd_drop<bf16_t, false>(a, stream);
 }

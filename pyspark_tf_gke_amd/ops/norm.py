@@ -146,8 +146,9 @@ def _like(x, dt, dev, n, strides, t, name):
 
 
 def _apart(o, on, size, ins):
-    """Output ``o`` may not overlap an input (pointer, name, whether the very same buffer will do).  Every
-    element is read before it is written, by the same thread."""
+    """Output ``o`` may not overlap an input (pointer, name, whether the very same buffer will do).  A value is
+    used by the thread that writes its place, and read before; the last lane of an unaligned row reads its
+    neighbour's values too, so there the waves of a row meet before they write."""
     for i, name, same in ins:
         if -size < o - i < size and i and not (o == i and same):
             raise ValueError(f"block_norm: {on} overlaps {name}")
