@@ -212,7 +212,7 @@ def block_norm_fwd(x, *, res=None, post=None, gate=None, scale: float = 1.0, dro
 def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1.0, drop=None, pre=None, du=None,
                    dh=None, dx=None, dres=None, dgate=None, dpost=None, dpre=None, workspace=None):
     """Gradients of :func:`block_norm_fwd` (same x, res, post, gate, scale, drop, pre) from ``du`` (with
-    ``pre``) and ``dh`` (None: zero).  Writes dx and dres (None: skipped), ``dgate`` like ``gate``, and
+    ``pre``) and ``dh`` (None: zero).  ``stats`` as that call left them (None where neither norm is there).  Writes dx and dres (None: skipped), ``dgate`` like ``gate``, and
     ``dpost`` / ``dpre`` = (dgamma, dbeta), fp32 [C] or None where the norm has none.  ``dx`` and ``dres``
     may each be one of x, res, du and dh; nothing else may overlap.  ``workspace``:
     :func:`block_norm_workspace` (None: allocated here)."""
@@ -231,7 +231,10 @@ def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1
     hp = _like(x, dt, dev, n, st, dh, "dh")
     dxp = _like(x, dt, dev, n, st, dx, "dx")
     drp = _like(x, dt, dev, n, st, dres, "dres")
-    _stats_ok(stats, M, dev)
+    if stats is not None:
+        _stats_ok(stats, M, dev)
+    elif k1 or k2:
+        raise ValueError("block_norm: the gradients of a norm need the forward pass's stats")
     if dgate is not None and (gate is None or dgate.shape != gate.shape or dgate.dtype is not gate.dtype
                               or dgate.get_device() != dev or not dgate.is_contiguous()):
         raise ValueError("block_norm: dgate must match gate")
@@ -282,7 +285,7 @@ def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1
         bits |= gp | dgp
     v = [0 if t is None else t.data_ptr() for t in vecs]
     hip_on(x.device, "ptg_block_norm_bwd",
-           _BWD.pack(xp, rp, gp, up, hp, dxp, drp, g1, b1, g2, stats.data_ptr(), *v, dgp, workspace.data_ptr(), d[5], M, C, f32,
+           _BWD.pack(xp, rp, gp, up, hp, dxp, drp, g1, b1, g2, 0 if stats is None else stats.data_ptr(), *v, dgp, workspace.data_ptr(), d[5], M, C, f32,
                      C % 8 == 0 and not bits & 15, k1, k2, mode, rpg, d[0], d[1], d[3], d[4], scale, d[2]))
     return dx, dres
 
@@ -363,7 +366,7 @@ def _ref_bwd(x, stats, res, post, gate, scale, drop, pre, du, dh, dx, dres, dgat
         if t is not None:
             t.copy_(v.reshape(t.shape).to(t.dtype))
 
-    m1, s1, m2, s2 = (stats[k].view(M, 1) for k in range(4))
+    m1, s1, m2, s2 = (0.0, 1.0, 0.0, 1.0) if stats is None else (stats[k].view(M, 1) for k in range(4))
     n = x.reshape(M, C).float()
     xh = (n - m1) * s1
     if post is not None:
