@@ -162,16 +162,14 @@ class BlockOp:
         d = _drop_now(self, dev) if training else None
         h = ws.get(self.name + "/h", x.shape, dt, dev) if self.want_h else None
         u = ws.get(self.name + "/u", x.shape, dt, dev) if self.pre is not None else None
-        M = x.numel() // x.shape[-1]
-        st = ws.get(self.name + "/stats", (4, M), torch.float32, dev) if training else None
+        st = None
+        if training and (self.post is not None or self.pre is not None):
+            st = ws.get(self.name + "/stats", (4, x.numel() // x.shape[-1]), torch.float32, dev)
         self._kw = dict(res=res, post=self._norm(self.post), gate=gate, scale=self.scale, drop=d,
                         pre=self._norm(self.pre))
         self._x, self._st, self._gshape = x, st, xs[1].shape if self.gate_input else None
         if self._wide(x):
-            if st is not None:
-                self._st = ws.get(self.name + "/stats", (4, self._flat(x).shape[0]), torch.float32, dev)
-            kw = self._wide_kw()
-            NM.block_norm_fwd(self._flat(x), h=self._flat(h), stats=self._st, **kw)
+            NM.block_norm_fwd(self._flat(x), h=self._flat(h), **self._wide_kw())
         else:
             NM.block_norm_fwd(x, h=h, u=u, stats=st, **self._kw)
         return [t for t in (h, u) if t is not None]
