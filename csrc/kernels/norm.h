@@ -37,7 +37,7 @@ struct FwdCall {
   const float *g1, *b1, *g2, *b2;
   float* stats;
   const void* step_dev;
-  int64_t M, C, f32, aligned, kind1, kind2, gate_mode, rpg, drop, thr, seed, step;
+  int64_t M, C, f32, aligned, kind1, kind2, gate_mode, rpg, drop, thr, seed, step, first;
   double eps1, eps2, scale, dscale;
 };
 struct BwdCall {
@@ -48,10 +48,10 @@ struct BwdCall {
   void* dgate;
   float* ws;
   const void* step_dev;
-  int64_t M, C, f32, aligned, kind1, kind2, gate_mode, rpg, drop, thr, seed, step;
+  int64_t M, C, f32, aligned, kind1, kind2, gate_mode, rpg, drop, thr, seed, step, first;
   double scale, dscale;
 };
-static_assert(sizeof(FwdCall) == 27 * 8 && sizeof(BwdCall) == 32 * 8, "64-bit fields");
+static_assert(sizeof(FwdCall) == 28 * 8 && sizeof(BwdCall) == 33 * 8, "64-bit fields");
 
 typedef __attribute__((ext_vector_type(4))) unsigned int vu4_t;
 
@@ -371,9 +371,9 @@ static inline int col_vec_bytes(int nt, int C, int n, const bool* there, int mos
 template <bool ALN>
 PTG_DEV void row_keep(const BlkArgs& a, uint64_t step, long at, uint32_t off, bool* k) {
   if (ALN) {
-    keep8(philox(((uint64_t)at >> 3) + (off >> 3), step, a.d.seed), a.d.thr, k);
+    keep8(philox((((uint64_t)at + a.d.first) >> 3) + (off >> 3), step, a.d.seed), a.d.thr, k);
   } else {
-    const uint32_t b = keep8_at((uint64_t)at + off, step, a.d);
+    const uint32_t b = keep8_at((uint64_t)at + a.d.first + off, step, a.d);
 #pragma unroll
     for (int j = 0; j < 8; ++j) k[j] = (b >> j) & 1u;
   }

@@ -422,7 +422,7 @@ int ptg_block_norm_bwd(const void* call, hipStream_t stream) {
   a.stats = c.stats;
   a.M = M; a.C = C; a.kind1 = kind1; a.kind2 = kind2;
   a.gate_mode = gate_mode; a.rpg = gate_mode == GATE_GROUP ? rpg : 1; a.scale = (float)c.scale; a.drop = (int)c.drop;
-  a.d = drop_args((int)c.thr, (float)c.dscale, c.seed, c.step, c.step_dev);
+  a.d = drop_args((int)c.thr, (float)c.dscale, c.seed, c.step, c.step_dev, c.first);
   a.dgate = dgate;
   auto over = [&](const void* o) { return o && (o == c.x || o == c.res || o == c.du || o == c.dh); };
   a.over = !aligned && (over(c.dx) || over(c.dres));

@@ -146,7 +146,7 @@ int fwd_drop(const BlkArgs& a, hipStream_t stream) {
 
 extern "C" {
 
-// call: a FwdCall.  aligned: every tensor starts on 16 bytes and C % 8 == 0.  Rows per gate group: rpg.
+// call: a FwdCall.  aligned: every tensor starts on 16 bytes, C % 8 == 0 and first % 8 == 0.  Rows per gate group: rpg.
 int ptg_block_norm_fwd(const void* call, hipStream_t stream) {
   const FwdCall& c = *(const FwdCall*)call;
   if (c.M <= 0) return 0;
@@ -158,7 +158,7 @@ int ptg_block_norm_fwd(const void* call, hipStream_t stream) {
   a.M = c.M; a.C = (int)c.C; a.kind1 = (int)c.kind1; a.kind2 = (int)c.kind2;
   a.eps1 = (float)c.eps1; a.eps2 = (float)c.eps2;
   a.gate_mode = (int)c.gate_mode; a.rpg = c.rpg > 0 ? c.rpg : 1; a.scale = (float)c.scale; a.drop = (int)c.drop;
-  a.d = drop_args((int)c.thr, (float)c.dscale, c.seed, c.step, c.step_dev);
+  a.d = drop_args((int)c.thr, (float)c.dscale, c.seed, c.step, c.step_dev, c.first);
   a.over = !c.aligned && c.h && (c.h == c.x || c.h == c.res);
   if (c.f32) return c.aligned ? fwd_drop<float, true>(a, stream) : fwd_drop<float, false>(a, stream);
   return c.aligned ? fwd_drop<bf16_t, true>(a, stream) : fwd_drop<bf16_t, false>(a, stream);

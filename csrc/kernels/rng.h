@@ -15,9 +15,10 @@ struct DropArgs {
   float scale;           // 1 / keep probability
   uint64_t seed, step;
   const long* step_dev;  // device-resident step (captured graphs), overrides `step`
+  uint64_t first;        // mask index of the tensor's first element
 };
-static inline DropArgs drop_args(int thr, float scale, long seed, long step, const void* step_dev) {
-  return DropArgs{(uint32_t)thr, scale, (uint64_t)seed, (uint64_t)step, (const long*)step_dev};
+static inline DropArgs drop_args(int thr, float scale, long seed, long step, const void* step_dev, long first = 0) {
+  return DropArgs{(uint32_t)thr, scale, (uint64_t)seed, (uint64_t)step, (const long*)step_dev, (uint64_t)first};
 }
 PTG_DEV uint64_t drop_step(const DropArgs& d) { return d.step_dev ? (uint64_t)*d.step_dev : d.step; }
 

@@ -27,8 +27,6 @@ from __future__ import annotations
 import time
 
 import numpy as np
-import math
-
 import torch
 
 from . import engine as E
@@ -136,9 +134,7 @@ def _add_into(ex, g) -> None:
     if ex.dtype == g.dtype == torch.bfloat16:
         KB.add_(ex, g, ex)
     else:
-        rows = (-1, math.gcd(ex.numel(), NM.MAX_COLS))  # elementwise: any rows will do
-        ex = ex.view(rows)
-        NM.block_norm_fwd(g.to(ex.dtype).contiguous().view(rows), res=ex, h=ex)
+        NM.flat_fwd(g.to(ex.dtype).contiguous(), res=ex, h=ex)
 
 
 def _lower(nodes: list, input_idx: int) -> list:

@@ -8,8 +8,6 @@ draws the dropout mask again instead of reading one.  Any part alone is the same
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from ..ops import dropout as DR
@@ -169,23 +167,15 @@ class BlockOp:
                         pre=self._norm(self.pre))
         self._x, self._st, self._gshape = x, st, xs[1].shape if self.gate_input else None
         if self._wide(x):
-            NM.block_norm_fwd(self._flat(x), h=self._flat(h), **self._wide_kw())
+            NM.flat_fwd(x, res=res, gate=gate, scale=self.scale, drop=d, h=h)
         else:
             NM.block_norm_fwd(x, h=h, u=u, stats=st, **self._kw)
         return [t for t in (h, u) if t is not None]
 
-    # Rows above the kernels' width, without a norm or a gate vector: elementwise, so any rows will do
-    # (the dropout mask goes by the element's index).
+    # Rows above the kernels' width, without a norm or a gate vector: elementwise.
     def _wide(self, x) -> bool:
         return x.shape[-1] > NM.MAX_COLS and self.post is None and self.pre is None and self.gate is None \
             and (not self.gate_input or self._kw["gate"].numel() == x.numel())
-
-    @staticmethod
-    def _flat(t):
-        return None if t is None else t.view(-1, math.gcd(t.numel(), NM.MAX_COLS))
-
-    def _wide_kw(self):
-        return {**self._kw, "res": self._flat(self._kw["res"]), "gate": self._flat(self._kw["gate"])}
 
     def _grads(self, layer):
         if layer is None:
@@ -214,17 +204,17 @@ class BlockOp:
             dgate = ws.get(self.name + "/dgate", kw["gate"].shape, dt, dev)
         elif self.gate is not None:
             dgate = self.gate.gamma.grad
-        wsp = None
-        fl = lambda t: t  # noqa: E731
         if self._wide(x):
-            fl, kw = self._flat, self._wide_kw()
-        if x.is_cuda:
-            C = fl(x).shape[-1]
-            M = x.numel() // C
-            G = kw["gate"].shape[0] if self.gate_input else 1
-            wsp = ws.get(self.name + "/colsums", (NM.block_norm_workspace_floats(M, C, G),), torch.float32, dev)
-        NM.block_norm_bwd(fl(x), st, du=du, dh=fl(dh), dx=fl(dx), dres=fl(dres), dgate=fl(dgate),
-                          dpost=self._grads(self.post), dpre=self._grads(self.pre), workspace=wsp, **kw)
+            NM.flat_bwd(x, gate=kw["gate"], scale=self.scale, drop=kw["drop"], dh=dh, dx=dx, dres=dres, dgate=dgate)
+        else:
+            wsp = None
+            if x.is_cuda:
+                C = x.shape[-1]
+                G = kw["gate"].shape[0] if self.gate_input else 1
+                floats = NM.block_norm_workspace_floats(x.numel() // C, C, G)
+                wsp = ws.get(self.name + "/colsums", (floats,), torch.float32, dev)
+            NM.block_norm_bwd(x, st, du=du, dh=dh, dx=dx, dres=dres, dgate=dgate, dpost=self._grads(self.post),
+                              dpre=self._grads(self.pre), workspace=wsp, **kw)
         return [dx] + ([dgate.view(self._gshape)] if self.gate_input else []) + ([dres] if self.res else [])
 
 

@@ -28,11 +28,13 @@ _CALL = struct.Struct("=3Q7qd")  # DropCall of dropout.hip
 
 
 class Drop(NamedTuple):
-    """A dropout inside a fused operator: rate, 64-bit seed, step (int or int64 device tensor)."""
+    """A dropout inside a fused operator: rate, 64-bit seed, step (int or int64 device tensor), and the mask
+    index of the tensor's first element (a part of a larger tensor draws that part of its mask)."""
 
     rate: float
     seed: int
     step: object = 0
+    first: int = 0
 
 
 def threshold(rate: float) -> tuple[int, float]:
@@ -114,13 +116,15 @@ def _pieces(blocks, step: int, seed: int):
     return torch.stack((w & 0xFFFF, w >> 16), 2).reshape(len(blocks), 8)
 
 
-def keep_mask(shape, rate: float, seed: int, step, noise_shape=None) -> torch.Tensor:
-    """The bool mask (host reference), of ``shape``."""
+def keep_mask(shape, rate: float, seed: int, step, noise_shape=None, first: int = 0) -> torch.Tensor:
+    """The bool mask (host reference), of ``shape``, from mask index ``first`` on."""
     thr, _ = threshold(rate)
     outer, mid, inner = noise_dims(shape, noise_shape)
     n = outer * inner
     step = int(step)
-    p = _pieces(torch.arange((n + 7) // 8, dtype=torch.int64), step, int(seed)).reshape(-1)[:n]
+    lo = first // 8
+    p = _pieces(torch.arange(lo, (first + n + 7) // 8, dtype=torch.int64), step, int(seed))
+    p = p.reshape(-1)[first - 8 * lo:first - 8 * lo + n]
     return (p >= thr).view(outer, 1, inner).expand(outer, mid, inner).reshape(tuple(shape))
 
 

@@ -32,8 +32,8 @@ MAX_COLS = 8192
 
 
 # arguments of the C entries: 64 bits each, as FwdCall and BwdCall of norm.h
-_FWD = struct.Struct("=11Q12q4d")
-_BWD = struct.Struct("=18Q12q2d")
+_FWD = struct.Struct("=11Q13q4d")
+_BWD = struct.Struct("=18Q13q2d")
 
 
 class Norm(NamedTuple):
@@ -63,7 +63,7 @@ def block_norm_workspace(rows: int, cols: int, groups: int, device) -> torch.Ten
     return torch.empty(block_norm_workspace_floats(rows, cols, groups), dtype=torch.float32, device=device)
 
 
-_NO_DROP = (0, 0, 1.0, 0, 0, 0)  # on, threshold, scale, seed, host step, device step's address
+_NO_DROP = (0, 0, 1.0, 0, 0, 0, 0)  # on, threshold, scale, seed, host step, device step's address, first index
 
 
 def _bad(name, x):
@@ -128,11 +128,18 @@ def _common(x, gate, drop):
             if M and (G == 0 or M % G):
                 raise ValueError(f"block_norm: {M} rows do not divide into {G} gate groups")
             mode, rpg = 2, M // G if G else 1
+    return M, C, dev, mode, rpg, _drop_args(drop, x.device)
+
+
+def _drop_args(drop, device):
     if drop is None:
-        return M, C, dev, mode, rpg, _NO_DROP
+        return _NO_DROP
     thr, ds = DR.threshold(drop.rate)
-    host, step = DR.step_args(drop.step, x.device)
-    return M, C, dev, mode, rpg, (1, thr, ds, DR._signed(drop.seed), host, 0 if step is None else step.data_ptr())
+    host, step = DR.step_args(drop.step, device)
+    first = int(drop.first)
+    if not 0 <= first < 1 << 62:
+        raise ValueError(f"block_norm: a mask begins at an index from 0 on, got {first}")
+    return 1, thr, ds, DR._signed(drop.seed), host, 0 if step is None else step.data_ptr(), first
 
 
 def _like(x, dt, dev, n, strides, t, name):
@@ -202,10 +209,10 @@ def block_norm_fwd(x, *, res=None, post=None, gate=None, scale: float = 1.0, dro
             stats.copy_(st)
         return h, u
     gp = 0 if gate is None else gate.data_ptr()
-    aligned = C % 8 == 0 and not (xp | rp | hp | up | (gp if mode == 2 else 0)) & 15
+    aligned = not ((C | d[6]) & 7 or (xp | rp | hp | up | (gp if mode == 2 else 0)) & 15)
     hip_on(x.device, "ptg_block_norm_fwd",
            _FWD.pack(xp, rp, gp, hp, up, g1, b1, g2, b2, 0 if stats is None else stats.data_ptr(), d[5], M, C, f32, aligned,
-                     k1, k2, mode, rpg, d[0], d[1], d[3], d[4], e1, e2, scale, d[2]))
+                     k1, k2, mode, rpg, d[0], d[1], d[3], d[4], d[6], e1, e2, scale, d[2]))
     return h, u
 
 
@@ -286,8 +293,100 @@ def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1
     v = [0 if t is None else t.data_ptr() for t in vecs]
     hip_on(x.device, "ptg_block_norm_bwd",
            _BWD.pack(xp, rp, gp, up, hp, dxp, drp, g1, b1, g2, 0 if stats is None else stats.data_ptr(), *v, dgp, workspace.data_ptr(), d[5], M, C, f32,
-                     C % 8 == 0 and not bits & 15, k1, k2, mode, rpg, d[0], d[1], d[3], d[4], scale, d[2]))
+                     not ((C | d[6]) & 7 or bits & 15), k1, k2, mode, rpg, d[0], d[1], d[3], d[4], d[6], scale, d[2]))
     return dx, dres
+
+
+# ---------------------------------------------------------------------------------------- without norms
+# Without a norm the pass is elementwise and takes tensors of any shape: as rows of 1024 columns (four a workgroup
+# of the backward pass, two of the forward), and what is left over as one row behind them, whose mask goes on where
+# theirs ends.  There is nothing to sum up, so the backward pass takes no workspace.
+FLAT_COLS = 1024
+
+
+def _flat_parts(n):
+    """(first element, rows, columns) of the launches"""
+    rows, rest = divmod(n, FLAT_COLS)
+    return ([(0, rows, FLAT_COLS)] if rows else []) + ([(n - rest, 1, rest)] if rest else [])
+
+
+def _flat_common(x):
+    dt = x.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float32:
+        raise TypeError(f"block_norm: expected bfloat16 or float32, got {dt}")
+    if not x.is_contiguous():
+        raise ValueError("block_norm: x must be contiguous")
+    return dt, x.get_device(), x.numel(), x.data_ptr(), x.element_size()
+
+
+def _flat_like(x, dt, dev, n, t, name):
+    if t is None:
+        return 0
+    if t.dtype is not dt or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        _bad(name, x)
+    return t.data_ptr()
+
+
+def flat_fwd(x, *, res=None, gate=None, scale: float = 1.0, drop=None, h):
+    """h = res + dropout(scale * gate * x) over tensors of any shape, as many values in each.  ``h`` may be ``res`` or
+    ``x``; nothing else may overlap.  Returns h."""
+    dt, dev, n, xp, size = _flat_common(x)
+    rp = _flat_like(x, dt, dev, n, res, "res")
+    gp = _flat_like(x, dt, dev, n, gate, "gate")
+    hp = _flat_like(x, dt, dev, n, h, "h")
+    d = _drop_args(drop, x.device)
+    _apart(hp, "h", n * size, ((xp, "x", True), (rp, "res", True), (gp, "gate", False)))
+    if dev < 0:
+        row = lambda t: None if t is None else t.reshape(1, n)  # noqa: E731
+        h.copy_(_ref_fwd(row(x), row(res), None, row(gate), scale, drop, None, 1, n, 1)[0].view(h.shape).to(dt))
+        return h
+    for lo, M, C in _flat_parts(n):
+        at = lambda p: p and p + lo * size  # noqa: E731
+        aligned = not ((C | d[6]) & 7 or (at(xp) | at(rp) | at(gp) | at(hp)) & 15)
+        hip_on(x.device, "ptg_block_norm_fwd",
+               _FWD.pack(at(xp), at(rp), at(gp), at(hp), 0, 0, 0, 0, 0, 0, d[5], M, C, size == 4, aligned, 0, 0,
+                         2 if gp else 0, 1, d[0], d[1], d[3], d[4], d[6] + lo, 0.0, 0.0, scale, d[2]))
+    return h
+
+
+def flat_bwd(x, *, gate=None, scale: float = 1.0, drop=None, dh, dx=None, dres=None, dgate=None):
+    """Gradients of :func:`flat_fwd`, written to those of dx, dres and dgate that are given.  ``dx`` and ``dres`` may
+    each be x or dh; nothing else may overlap."""
+    dt, dev, n, xp, size = _flat_common(x)
+    gp = _flat_like(x, dt, dev, n, gate, "gate")
+    hp = _flat_like(x, dt, dev, n, dh, "dh")
+    dxp = _flat_like(x, dt, dev, n, dx, "dx")
+    drp = _flat_like(x, dt, dev, n, dres, "dres")
+    dgp = _flat_like(x, dt, dev, n, dgate, "dgate")
+    d = _drop_args(drop, x.device)
+    if dh is None:
+        raise ValueError("block_norm: no gradient comes in (dh is None)")
+    if dx is None and dres is None and dgate is None:
+        raise ValueError("block_norm: no gradient is asked for")
+    if dgate is not None and gate is None:
+        raise ValueError("block_norm: dgate must match gate")
+    ins, bytes_ = ((xp, "x", True), (hp, "dh", True), (gp, "gate", False)), n * size
+    for p, name in ((dxp, "dx"), (drp, "dres")):
+        if p:
+            _apart(p, name, bytes_, ins)
+    if dxp and drp:
+        _apart(drp, "dres", bytes_, ((dxp, "dx", False),))
+    if dgp:
+        _apart(dgp, "dgate", bytes_, [(p, name, False) for p, name, _ in ins] + [(dxp, "dx", False), (drp, "dres", False)])
+    if dev < 0:
+        row = lambda t: None if t is None else t.view(1, n)  # noqa: E731
+        _ref_bwd(row(x), None, None, None, row(gate), scale, drop, None, None, row(dh), row(dx), row(dres), row(dgate),
+                 (None,) * 4, 1, n, 1)
+        return
+    if gate is not None and dgate is None:
+        dgate = torch.empty_like(gate)  # written all the same
+        dgp = dgate.data_ptr()
+    for lo, M, C in _flat_parts(n):
+        at = lambda p: p and p + lo * size  # noqa: E731
+        aligned = not ((C | d[6]) & 7 or (at(xp) | at(gp) | at(hp) | at(dxp) | at(drp) | at(dgp)) & 15)
+        hip_on(x.device, "ptg_block_norm_bwd",
+               _BWD.pack(at(xp), 0, at(gp), 0, at(hp), at(dxp), at(drp), 0, 0, 0, 0, 0, 0, 0, 0, at(dgp), 0, d[5], M, C,
+                         size == 4, aligned, 0, 0, 2 if gp else 0, 1, d[0], d[1], d[3], d[4], d[6] + lo, scale, d[2]))
 
 
 _WS: dict = {}
@@ -328,7 +427,7 @@ def _ref_parts(x, gate, drop, M, C, rpg):
     keep = ks = None
     if drop is not None:
         _, ks = DR.threshold(drop.rate)
-        keep = DR.keep_mask((M, C), drop.rate, drop.seed, drop.step)
+        keep = DR.keep_mask((M, C), drop.rate, drop.seed, drop.step, first=int(drop.first))
     return g, keep, ks
 
 
