@@ -254,7 +254,9 @@ __global__ __launch_bounds__(512) void int4_tile_k(Args4 a, int mb, int nbk, int
     xt[j] = min(nk, (a.K - k + QT_K - 1) / QT_K);
     wo[j] = ((uint32_t)(wid * 2 + j) * (uint32_t)kt + (uint32_t)t0) * 1024u + (uint32_t)lane * 16u;
   }
-  // stages past the end are issued too, out of range (zeros, no traffic): the count of loads in flight stays known
+  // stages past the end are issued too, out of range (zeros, no traffic): the count of loads in flight stays known.
+  // So does their order, by the barrier behind each: q_wait_vm counts on the stages arriving one after another,
+  // and to the scheduler their places in LDS have nothing to do with each other.
   auto issue = [&](int t, unsigned char* base) {
     base += wid * 2048;
 #pragma unroll
@@ -265,6 +267,7 @@ __global__ __launch_bounds__(512) void int4_tile_k(Args4 a, int mb, int nbk, int
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (q_lds_t*)(base + Q_XB + j * 1024), 16, wo[j] + wt, 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
   };
   const bf16_t* sp_[4];  // this lane's scales and zero points of the next stage
   const uint8_t* zp_[4];
@@ -306,7 +309,6 @@ __global__ __launch_bounds__(512) void int4_tile_k(Args4 a, int mb, int nbk, int
     scales(t + 2 + half);
     issue(t + QR - 2, f0);
     issue(t + QR - 1, f1);
-    __builtin_amdgcn_sched_barrier(0);
     const unsigned char* sx = st + n16 * 256;
     U4 wv[4];
 #pragma unroll
