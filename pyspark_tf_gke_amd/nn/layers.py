@@ -132,6 +132,7 @@ class Dense(Layer):
         self.fan_in = fin
         self.kernel = store.add(f"{self.name}/kernel", (self.units, fin), glorot_uniform(fin, self.units))
         self.params = [self.kernel]
+        self._store = store
         if self.use_bias:
             self.bias = store.add(f"{self.name}/bias", (self.units,), zeros)
             self.params.append(self.bias)
@@ -165,6 +166,7 @@ class Dense(Layer):
         from ..ops import quant as Q
 
         self.int4 = Q.int4_layout(codes, scale, zero, group)
+        self._store.quantized = True
         self.quantization = {"mode": "int4", "block_size": int(group), "zero_point": zero is not None}
         w = Q.int4_dequantize(self.int4)
         self.kernel.data.copy_(w)

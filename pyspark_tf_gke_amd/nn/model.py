@@ -99,7 +99,6 @@ class Sequential:
         self._eval_stats = None
         self.stop_training = False
         self.strategy = None
-        self._quantized = False
         for l in layers or []:
             self.add(l)
 
@@ -160,7 +159,7 @@ class Sequential:
     @property
     def quantized(self) -> bool:
         """Some layer runs on 4-bit weights: the model is for inference."""
-        return self._quantized
+        return self.store is not None and self.store.quantized
 
     def quantize(self, mode: str = "int4", block_size: int = 128, zero_point: bool = False) -> None:
         """Keras ``model.quantize("int4")``: every Dense layer of more than 64 units (a multiple of 8) whose
@@ -189,12 +188,11 @@ class Sequential:
                              f"{block_size} inputs")
         for l in todo:
             l.quantize(mode, block_size, zero_point)
-        self._quantized = True
         self.store.flip_token = None
         self._graphs, self._graph_warm = {}, {}  # captured training steps
 
     def _refuse_quantized(self, what: str) -> None:
-        if self._quantized:
+        if self.quantized:
             raise RuntimeError(f"{what}: the model is quantized (inference only)")
 
     def set_weights(self, ws):
@@ -943,7 +941,6 @@ def load_model(filepath: str, compile: bool = True, device=None) -> Sequential:
     m.build(device=device)
     for l in m.layers:
         l.load_weights(lambda k, n=l.name: tensors.get(f"layers/{n}/vars/{k}"))
-    m._quantized = any(getattr(l, "int4", None) is not None for l in m.layers)
     m.store.refresh_bf16()
     cc = cfg.get("compile_config") or {}
     if compile and cc.get("loss"):

@@ -75,6 +75,7 @@ class ParamStore:
     # filters (nn.optimizers.Adam.finish_fused); any other write to the weights clears it
     flip_token: tuple | None = None
     flip_names: frozenset = frozenset()
+    quantized: bool = False  # a layer runs on 4-bit weights: its master only shows what they stand for
 
     def add(self, name: str, shape, init, overwrite_grad=False, logical_numel=None, mask_fn=None) -> Param:
         p = Param(name, tuple(int(s) for s in shape), init, overwrite_grad, logical_numel, len(self.params),

@@ -140,6 +140,5 @@ def load(export_dir: str, device=None) -> LoadedModel:
     tensors = load_file(os.path.join(export_dir, "variables", "variables.safetensors"))
     for l in m.layers:
         l.load_weights(lambda k, n=l.name: tensors.get(f"{n}/{k}"))
-    m._quantized = any(getattr(l, "int4", None) is not None for l in m.layers)
     m.store.refresh_bf16()
     return LoadedModel(m, meta)
