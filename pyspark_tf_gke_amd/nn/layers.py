@@ -644,6 +644,11 @@ class Multiply(Layer):
         a, g = s
         if tuple(g) != tuple(a) and tuple(g) != (a[-1],):
             raise ValueError(f"Multiply: a gate of shape {g} does not fit a branch of shape {a}")
+        if tuple(g) != tuple(a):
+            from ..ops.norm import MAX_COLS
+
+            if a[-1] is not None and a[-1] > MAX_COLS:
+                raise NotImplementedError(f"Multiply: a gate row of at most {MAX_COLS} channels, got {a[-1]}")
         return tuple(a)
 
 
