@@ -9,9 +9,10 @@ the inverse of that exact keep probability.  Dropped elements are 0 whatever the
 ``step`` is a host integer or a one-element int64 device tensor that the kernel reads (a captured HIP
 graph then draws another mask every replay, see :func:`drop_advance`).
 
-``noise_shape`` (Keras): the shape of the mask, 1 (or None) on ONE run of axes that share an entry,
-e.g. ``(N, 1, 1, C)`` or ``(N, 1)``; None draws an entry per element.  GPU tensors run the kernel, CPU
-tensors the reference below.
+``noise_shape`` (Keras): the shape of the mask, 1 on ONE run of axes that share an entry, e.g. ``(N, 1, 1, C)``
+or ``(N, 1)``.  None on an axis is the input's own size there, ``(None, 1, 1, None)`` an entry for each
+sample and channel; None in place of the shape draws an entry per element.  GPU tensors run the kernel,
+CPU tensors the reference below.
 """
 from __future__ import annotations
 
