@@ -51,15 +51,21 @@ def int4_quantize(w: torch.Tensor, group: int = 128, zero_point: bool = False):
     g = w.detach().float().view(N, K // group, group)
     if zero_point:
         lo, hi = g.amin(2).clamp_max(0.0), g.amax(2).clamp_min(0.0)
-        scale = _bf16_up((hi - lo) / 15.0)
-        inv = torch.where(scale > 0, 1.0 / scale.float(), 0.0)
-        zero = torch.round(-lo * inv).clamp_(0, 15)
+        width = hi - lo
+        scale = _bf16_up(torch.where(torch.isfinite(width), width / 15.0, hi / 15.0 - lo / 15.0))
+        zero = torch.round(_steps(-lo, scale)).clamp_(0, 15)
     else:
         scale = _bf16_up(g.abs().amax(2) / 7.0)
-        inv = torch.where(scale > 0, 1.0 / scale.float(), 0.0)
-        zero = torch.full_like(inv, 8.0)
-    q = (torch.round(g * inv[:, :, None]) + zero[:, :, None]).clamp_(0, 15).to(torch.uint8).view(N, K)
+        zero = torch.full_like(scale, 8.0, dtype=torch.float32)
+    q = (torch.round(_steps(g, scale[:, :, None])) + zero[:, :, None]).clamp_(0, 15).to(torch.uint8).view(N, K)
     return q[:, 0::2] | (q[:, 1::2] << 4), scale, zero.to(torch.uint8) if zero_point else None
+
+
+def _steps(v, scale):
+    """v / scale, 0 where the scale is; a scale below 2**-128 has no fp32 reciprocal."""
+    s = scale.float()
+    inv = torch.where(s > 0, 1.0 / s, 0.0)
+    return torch.where(torch.isfinite(inv), v * inv, v / s)
 
 
 def _bf16_up(t):
