@@ -164,8 +164,8 @@ PTG_DEV void row_stats(const float* f, int nv, float layer, float eps, RowX& rx,
 // lane.  Otherwise a group is one unaligned vector load as well: the last group of a row reads the row's
 // last 8 values and is shifted down where it is used, a lane without columns or row reads the tensor's
 // first 8 and takes 0.  A branch around the load would wait for it there and then (1537 x 771 fp32
-// backward: 15.6 instead of 15.0 us).  Rows below 8 columns have no 8 values to read; they are among those of two lanes (TINY, up
-// to 16 columns), which load value by value.
+// backward: 15.6 instead of 15.0 us).  Rows below 8 columns have no 8 values to read; they are among those of two
+// lanes (TINY, up to 16 columns), which load value by value.
 template <typename T> struct Raw8;
 template <> struct Raw8<bf16_t> {
   U4 v;

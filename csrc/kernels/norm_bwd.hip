@@ -10,8 +10,12 @@
 // workgroups' partial sums in a fixed order: no atomics, the same bits every run.  As in the forward pass
 // the next row's loads are in flight while a row is worked on.
 //
-// Bound by HBM where it has rows enough (32768 x 2048 bf16: 151 us, 5.3 TB/s), by vector issue on the way there
-// (4096 x 1024 with both norms, gate and dropout: 17.8 us, 480 vector instructions a row of a wave, 80 % busy).
+// Bound by HBM where it has rows enough (32768 x 2048 bf16: 155 to 159 us, 5.1 TB/s).  On the way there a wave sees few
+// rows, so its start (vectors to LDS, first loads) and its end (five vectors joined) weigh as much as the rows: 4096 x
+// 1024 with both norms, gate and dropout, 4 rows a wave, takes 17.8 us, in which the vector pipes are 52 % busy
+// and the waves wait for 46 % of their time; 1537 x 771 fp32 with 53 gate rows, 2 rows a wave, 15.2 us, 33 % and 54 %.
+// Rows above 2048 columns take 16 waves of 128 registers, which are too few: 34 of the 48 such variants spill, up to
+// 89 registers with both norms (4096 x 8192 with all parts: bf16 173 us, 2.3 TB/s, fp32 332 us, 2.4 TB/s).
 #include "norm.h"
 
 // A thread's column sums over the rows (slots) of the workgroup: put_cols leaves them in LDS, [rows][cols]

@@ -1,6 +1,6 @@
 // Block norm, forward (norm.h): d = drop(scale * gate * post(x)); h = res + d; u = pre(h).
 //
-// Bound by HBM (32768 x 2048 bf16: 100 us, 5.4 TB/s; 4096 x 1024, 12.7 us, by its start and its end): x and res
+// Bound by HBM (32768 x 2048 bf16: 99 us, 5.4 TB/s; 4096 x 1024, 12.7 us, by its start and its end): x and res
 // in, h and u out, each once; statistics, the gate, the dropout mask and both
 // affine maps live in registers between the load and the stores of a row.  The next row's loads are
 // issued before the current row is worked on, so the row sums (and the barrier of rows of several waves)
@@ -110,8 +110,9 @@ __global__ __launch_bounds__(NT) void block_norm_fwd_k(BlkArgs a) {
 
 namespace {
 // Four waves a SIMD; three for rows above 1024 columns, which read more rows at a time as it is (32768 x 2048,
-// forward and backward together: 276 us with four, 259 with three; 401408 x 64: 56.9 with four, 58.2 with three).  Above 2048 columns a workgroup is 16 waves, one a CU (4096 x 8192 forward:
-// 73.7 us; 76.6 with two a CU, 93.9 on three quarters of the CUs).
+// forward and backward together: 276 us with four, 259 with three; 401408 x 64: 56.9 with four, 58.2 with three).
+// Above 2048 columns a workgroup is 16 waves, one a CU (4096 x 8192 forward: 73.7 us; 76.6 with two a CU, 93.9 on
+// three quarters of the CUs).
 template <typename T, bool ALN, bool PO, bool PR, bool DROP>
 int fwd_launch(const BlkArgs& a, hipStream_t stream) {
   auto go = [&](auto kern, int nt, int tpr) {
@@ -135,7 +136,8 @@ int fwd_launch(const BlkArgs& a, hipStream_t stream) {
 }
 template <typename T, bool ALN, bool DROP>
 int fwd_kind(const BlkArgs& a, hipStream_t stream) {
-  if (a.kind1) return a.kind2 ? fwd_launch<T, ALN, true, true, DROP>(a, stream) : fwd_launch<T, ALN, true, false, DROP>(a, stream);
+  if (a.kind1 && a.kind2) return fwd_launch<T, ALN, true, true, DROP>(a, stream);
+  if (a.kind1) return fwd_launch<T, ALN, true, false, DROP>(a, stream);
   return a.kind2 ? fwd_launch<T, ALN, false, true, DROP>(a, stream) : fwd_launch<T, ALN, false, false, DROP>(a, stream);
 }
 template <typename T, bool ALN>

@@ -79,8 +79,9 @@ PTG_DEV void int4_finish(const Args4& a, int m, int n, float s) {
 
 }  // namespace
 
-// Up to 32 rows, and small products: bound by reading the weights once (16 x 8192 x 8192: 12.5 us, 3 TB/s,
-// of which about 2 us pass before the first data are there).  A wave computes 16 * MT rows x 16 * NT outputs over its
+// Up to 32 rows, and small products: bound by reading the weights once (16 x 8192 x 8192: 12.8 us a pass among
+// others, 2.9 TB/s, 14.6 in the median where launches are traced; about 2 us pass before the first data are there,
+// and the waves wait for 77 % of their time).  A wave computes 16 * MT rows x 16 * NT outputs over its
 // share of K; the NW waves of a workgroup take the tiles of the workgroup's K range in turn and are joined
 // in LDS in a fixed order.  A product tile is one MFMA chain: sum (16 + u) x on top of -(16 + z) * sum x,
 // the latter from one MFMA with ones for every 32 inputs that all NT tiles share.  Waves that need few
@@ -217,7 +218,8 @@ __global__ __launch_bounds__(NW * 64) void int4_mm_k(Args4 a, int splits) {
 }
 
 // Larger products of more than 32 rows are bound by the matrix cores and by what feeds them, not by HBM: 256 x
-// 2048 x 20480 takes 32 us and 5 for the join, 670 TFLOP/s.  A pair of stages costs 5000 cycles, of which the two
+// 2048 x 20480 takes 32 us and 5 for the join, 670 TFLOP/s, with the matrix cores 42 % and the vector pipes 52 %
+// busy.  A pair of stages costs 5000 cycles, of which the two
 // waves' MFMAs are 2560 and their decoding, scaling and sums 2300: they overlap little.  A workgroup
 // takes 64 rows x 256 outputs; 4 waves hold 64 x 64 of them each, twice over: waves 4..7 work on every
 // other stage of 128 inputs, so two waves share a SIMD and one multiplies while the other waits, and the

@@ -479,7 +479,8 @@ class Dropout(Layer):
     rest scaled up; identity in inference.  The mask comes from a counter-based generator over (seed,
     training step, element) and is never stored.  ``noise_shape`` (batch axis included): 1 where the
     axis shares a mask entry, None where it has its own size, e.g. ``(None, 1, 1, None)`` for whole channels of
-    each sample; one run of axes may be shared.  ``seed`` None derives one from the weight-initialisation seed and the layer's name."""
+    each sample; one run of axes may be shared.  ``seed`` None derives one from the weight-initialisation
+    seed and the layer's name."""
 
     kind = "Dropout"
     keras_class = "Dropout"

@@ -123,7 +123,8 @@ def _common(x, gate, drop):
         else:
             if gate.dim() != 2 or gate.shape[1] != C or gate.dtype is not dt or gate.get_device() != dev \
                     or not gate.is_contiguous():
-                raise ValueError(f"block_norm: gate must be fp32 [{C}] or {dt} [groups, {C}], contiguous, on the device of x")
+                raise ValueError(f"block_norm: gate must be fp32 [{C}] or {dt} [groups, {C}], contiguous, on the "
+                                 "device of x")
             G = gate.shape[0]
             if M and (G == 0 or M % G):
                 raise ValueError(f"block_norm: {M} rows do not divide into {G} gate groups")
@@ -211,15 +212,16 @@ def block_norm_fwd(x, *, res=None, post=None, gate=None, scale: float = 1.0, dro
     gp = 0 if gate is None else gate.data_ptr()
     aligned = not ((C | d[6]) & 7 or (xp | rp | hp | up | (gp if mode == 2 else 0)) & 15)
     hip_on(x.device, "ptg_block_norm_fwd",
-           _FWD.pack(xp, rp, gp, hp, up, g1, b1, g2, b2, 0 if stats is None else stats.data_ptr(), d[5], M, C, f32, aligned,
-                     k1, k2, mode, rpg, d[0], d[1], d[3], d[4], d[6], e1, e2, scale, d[2]))
+           _FWD.pack(xp, rp, gp, hp, up, g1, b1, g2, b2, 0 if stats is None else stats.data_ptr(), d[5], M, C, f32,
+                     aligned, k1, k2, mode, rpg, d[0], d[1], d[3], d[4], d[6], e1, e2, scale, d[2]))
     return h, u
 
 
 def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1.0, drop=None, pre=None, du=None,
                    dh=None, dx=None, dres=None, dgate=None, dpost=None, dpre=None, workspace=None):
     """Gradients of :func:`block_norm_fwd` (same x, res, post, gate, scale, drop, pre) from ``du`` (with
-    ``pre``) and ``dh`` (None: zero).  ``stats`` as that call left them (None where neither norm is there).  Writes dx and dres (None: skipped), ``dgate`` like ``gate``, and
+    ``pre``) and ``dh`` (None: zero).  ``stats`` as that call left them (None where neither norm is there).
+    Writes dx and dres (None: skipped), ``dgate`` like ``gate``, and
     ``dpost`` / ``dpre`` = (dgamma, dbeta), fp32 [C] or None where the norm has none.  ``dx`` and ``dres``
     may each be one of x, res, du and dh; nothing else may overlap.  ``workspace``:
     :func:`block_norm_workspace` (None: allocated here)."""
@@ -292,8 +294,9 @@ def block_norm_bwd(x, stats, *, res=None, post=None, gate=None, scale: float = 1
         bits |= gp | dgp
     v = [0 if t is None else t.data_ptr() for t in vecs]
     hip_on(x.device, "ptg_block_norm_bwd",
-           _BWD.pack(xp, rp, gp, up, hp, dxp, drp, g1, b1, g2, 0 if stats is None else stats.data_ptr(), *v, dgp, workspace.data_ptr(), d[5], M, C, f32,
-                     not ((C | d[6]) & 7 or bits & 15), k1, k2, mode, rpg, d[0], d[1], d[3], d[4], d[6], scale, d[2]))
+           _BWD.pack(xp, rp, gp, up, hp, dxp, drp, g1, b1, g2, 0 if stats is None else stats.data_ptr(), *v, dgp,
+                     workspace.data_ptr(), d[5], M, C, f32, not ((C | d[6]) & 7 or bits & 15), k1, k2, mode, rpg,
+                     d[0], d[1], d[3], d[4], d[6], scale, d[2]))
     return dx, dres
 
 
@@ -372,7 +375,8 @@ def flat_bwd(x, *, gate=None, scale: float = 1.0, drop=None, dh, dx=None, dres=N
     if dxp and drp:
         _apart(drp, "dres", bytes_, ((dxp, "dx", False),))
     if dgp:
-        _apart(dgp, "dgate", bytes_, [(p, name, False) for p, name, _ in ins] + [(dxp, "dx", False), (drp, "dres", False)])
+        outs = ((dxp, "dx", False), (drp, "dres", False))
+        _apart(dgp, "dgate", bytes_, [(p, name, False) for p, name, _ in ins] + list(outs))
     if dev < 0:
         row = lambda t: None if t is None else t.view(1, n)  # noqa: E731
         _ref_bwd(row(x), None, None, None, row(gate), scale, drop, None, None, row(dh), row(dx), row(dres), row(dgate),

@@ -123,7 +123,8 @@ def int4_layout(codes, scale, zero=None, group: int = 128) -> Int4Weight:
         if (Np, Kp) != (N, K):
             p = torch.zeros((Np, Kp // group), dtype=t.dtype, device=t.device)
             p[:N, : K // group] = t
-        return p.view(Np // 16, 16, Kp // 128, 128 // group).permute(0, 2, 1, 3).clone(memory_format=torch.contiguous_format)
+        p = p.view(Np // 16, 16, Kp // 128, 128 // group).permute(0, 2, 1, 3)
+        return p.clone(memory_format=torch.contiguous_format)
 
     return Int4Weight(tiles, group_rows(scale), group_rows(zero), N, K, group)
 

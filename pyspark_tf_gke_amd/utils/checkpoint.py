@@ -1,7 +1,7 @@
 """Checkpoint / resume.  The reference only saves the final ``model.keras``; here a
 checkpoint holds the fp32 parameters (per parameter name), the optimizer state (Adam moments / SGD velocity) and
-step, the BatchNormalization moving statistics, the step of the dropout masks, the epoch, and every rank's RNG state, written
-atomically with safetensors + a JSON manifest.  Parameters/moments are stored once, per parameter
+step, the BatchNormalization moving statistics, the step of the dropout masks, the epoch, and every rank's RNG
+state, written atomically with safetensors + a JSON manifest.  Parameters/moments are stored once, per parameter
 name, in the full layout (rank 0 writes them after the strategy gathered any sharded state); each
 rank writes its own RNG file.
 """
@@ -64,7 +64,8 @@ def save_checkpoint(model, path: str, epoch: int, extra: dict | None = None) -> 
     comm.barrier()
     if rank == 0:
         manifest = {"epoch": epoch, "step": opt.iterations if opt else 0, "world_size": comm.world_size(),
-                    "drop_step": _drop_step(model), "sharded": False, "layout": "per-param", "total": int(st.total), "time": time.time(),
+                    "drop_step": _drop_step(model), "sharded": False, "layout": "per-param",
+                    "total": int(st.total), "time": time.time(),
                     **(extra or {})}
         with open(os.path.join(path, "manifest.json.tmp"), "w") as fh:
             json.dump(manifest, fh)
