@@ -115,3 +115,30 @@ def test_images_rescaled_in_front_train_on_the_gpu(hip_built):
     for _ in range(2):
         assert np.isfinite(m.train_on_batch(x, y)[0])
     assert all(np.abs(a - b).max() > 0 for a, b in zip(before, m.get_weights()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("functional", [False, True])
+def test_first_convolution_takes_its_own_path_behind_a_rescaling(hip_built, functional):
+    """Halving is exact in bf16: the model with a Rescaling(0.5) is the one without it on halved images."""
+
+    def model(front):
+        L.reset_name_counters()
+        ls = [*front, nn.Conv2D(8, 5, padding="same", name="c0"), nn.PReLU(name="p0"), nn.MaxPooling2D(name="m0"),
+              nn.Conv2D(16, 5, padding="same", name="c1"), nn.PReLU(name="p1"), nn.MaxPooling2D(name="m1"),
+              nn.GlobalAveragePooling2D(name="gap"), nn.Dense(2, name="head")]
+        if not functional:
+            return compiled(nn.Sequential([nn.Input(shape=(32, 40, 3)), *ls]), "cuda")
+        inp = t = nn.Input(shape=(32, 40, 3))
+        for l in ls:
+            t = l(t)
+        return compiled(nn.Model(inp, t), "cuda")
+
+    x, y = images(16, (32, 40, 3))
+    a, ga = engine_grads(model([nn.Rescaling(0.5, name="r")]), x, y)
+    b, gb = engine_grads(model([]), 0.5 * x, y)
+    assert torch.equal(a, b)
+    # the same kernels on the same numbers: only the order of fp32 sums over workgroups may differ, by at most
+    # 16 * 32 * 40 terms * 2**-24 = 1.3e-3 of their magnitudes, which may cancel to some share of themselves
+    for k in ga:
+        assert float((ga[k] - gb[k]).norm()) <= 1e-2 * float(gb[k].norm()), k
